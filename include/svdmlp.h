@@ -534,6 +534,123 @@ int svdmlp_forward_partial_f16_peer(const svdmlp_layout* layout, const void* pac
 int svdmlp_peer_sum_f16(void* const* bases, int world, int rank, int64_t off_slots, int slot_rows, int m, int c,
                         int64_t ld_slot, void* out, int64_t ld_out, void* stream);
 
+/* ------------------------------------------------- attention and its cache
+ *
+ * The attention half of a decoder layer, beside the MLP above: rotary
+ * positions with the cache write, attention over packed prompts, attention of
+ * a few new tokens per request over the paged cache, and the step that turns
+ * request lengths into block tables and slots.  The reference runs these in
+ * JAX around its MLP (models/modeling_llama.py: RoPE, KV cache, GQA attention;
+ * bench/e2e_block.py:208-229).
+ *
+ * Activations are 16-bit (dtype below) tensors [tokens, heads, head_dim] with
+ * strides in elements for tokens and heads and a unit stride inside a head, so
+ * that q, k and v may be views of one projection's output.  The cache of one
+ * layer is two tensors [num_blocks, kv_heads, block_size, head_dim], contiguous
+ * inside a block, with a stride in elements between blocks.  A slot names one
+ * token's place: block * block_size + offset.  Query head h reads key/value
+ * head h / (q_heads / kv_heads).
+ *
+ * Offsets and tables that live on the device are never trusted: a request's
+ * rows are clipped to the tensor, a block or slot outside the cache is not
+ * touched. */
+#define SVDMLP_BF16 0
+#define SVDMLP_F16 1
+
+/* Rotary positions and the cache write.  The first rotary_dim elements of
+ * every head of q and k are turned by angle positions[t] * inv_freq[i], pair i
+ * being elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; the
+ * turned elements are multiplied by `scale` (the magnitude of a stretched
+ * context), the rest of the head is copied.  k (turned) and v go to
+ * slots[t] of the caches; a token whose slot is negative, or beyond the cache,
+ * is written nowhere.  k_out may be NULL; k_cache and v_cache may both be
+ * NULL (then v and slots are not read).  q_out and k_out are contiguous and
+ * may be q and k themselves when those are contiguous. */
+typedef struct svdmlp_rope_args {
+  int32_t dtype, tokens, q_heads, kv_heads, head_dim, rotary_dim, interleaved;
+  int32_t block_size, num_blocks;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides */
+  const int32_t* positions;                                  /* [tokens] */
+  const int64_t* slots;                                      /* [tokens] */
+  const float* inv_freq;                                     /* [rotary_dim / 2] */
+  void *q_out, *k_out;
+  void *k_cache, *v_cache;
+  int64_t k_block, v_block; /* strides between blocks */
+} svdmlp_rope_args;
+int svdmlp_rope(const svdmlp_rope_args* args, void* stream);
+
+/* Block tables, slots and positions of one forward pass.  Request b holds
+ * held[b] tokens and adds added[b]; it needs ceil((held + added) / block_size)
+ * blocks, at most table_width.  The blocks it lacks come off the end of
+ * free_blocks[0 .. *free_count), requests in order, and are entered into
+ * table[b].  Outputs: slots[t] and positions[t] of the `tokens` new tokens,
+ * packed in request order (entries beyond the sum of added: slot -1, position
+ * 0), cu[0 .. batch] their offsets, lens[b] = held + added, *count_out what is
+ * left of the free list, *missing the blocks that it lacked (their entries and
+ * slots are -1).  Only new table entries are written: the call may be
+ * repeated.  Negative lengths count as 0. */
+typedef struct svdmlp_pages_args {
+  int32_t batch, tokens, block_size, table_width, free_capacity, reserved;
+  int32_t* table; /* [batch, ld_table] */
+  int64_t ld_table;
+  const int32_t *held, *added, *free_blocks, *free_count;
+  int64_t* slots;
+  int32_t *positions, *cu, *lens, *count_out, *missing;
+} svdmlp_pages_args;
+int svdmlp_page_step(const svdmlp_pages_args* args, void* stream);
+
+/* Attention over packed sequences.  Sequence b has the query rows
+ * [cu_q[b], cu_q[b + 1]) and the keys [cu_k[b], cu_k[b + 1]); when causal,
+ * query i of n sees the first m - n + i + 1 of m keys (the queries are the last
+ * n tokens).  out = softmax(scale q k^T) v; a row that sees no key gives zeros.
+ * head_dim is 64 or 128; rows and heads 16-byte aligned.  `workspace`: at least
+ * svdmlp_prompt_workspace_bytes, initialised by svdmlp_workspace_init. */
+typedef struct svdmlp_prompt_args {
+  int32_t dtype, batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, causal;
+  float scale;
+  int32_t reserved;
+  const void *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  const int32_t *cu_q, *cu_k; /* [batch + 1] */
+  void* out;
+  int64_t out_token, out_head;
+  void* workspace;
+  int64_t workspace_bytes;
+} svdmlp_prompt_args;
+int64_t svdmlp_prompt_workspace_bytes(void);
+int svdmlp_prompt_attention(const svdmlp_prompt_args* args, void* stream);
+
+/* Attention of each request's newest tokens over the paged cache, their own
+ * keys and values included (written before: svdmlp_rope).  Request b has the
+ * query rows [cu_q[b], cu_q[b + 1]), n of them, and lens[b] tokens in the
+ * cache, the newest n being its tree.  Every row sees the context (the first
+ * lens - n); in the tree, row i sees tree token j when bit j of mask[row] is
+ * set, or, with mask NULL, when j <= i (a chain; n = 1 is ordinary decoding).
+ * A mask names the first 64 tree tokens only.  max_tree, the largest n the
+ * caller expects, sizes the tiles; larger trees are still computed. */
+typedef struct svdmlp_tree_args {
+  int32_t dtype, batch, tokens, q_heads, kv_heads, head_dim;
+  int32_t block_size, num_blocks, table_width, max_tree;
+  float scale;
+  int32_t reserved;
+  const void* q;
+  int64_t q_token, q_head;
+  const void *k_cache, *v_cache;
+  int64_t k_block, v_block;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t *lens, *cu_q;
+  const int64_t* mask; /* [tokens] or NULL */
+  void* out;
+  int64_t out_token, out_head;
+  void* workspace;
+  int64_t workspace_bytes;
+} svdmlp_tree_args;
+int64_t svdmlp_tree_workspace_bytes(int32_t head_dim);
+int svdmlp_tree_attention(const svdmlp_tree_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

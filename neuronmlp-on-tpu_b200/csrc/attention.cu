@@ -1,0 +1,219 @@
+// Host side of the attention operators: argument checks and launches.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/svdmlp.h"
+#include "attention_rows.cuh"
+#include "host.h"
+#include "rope_pages.cuh"
+
+namespace svdmlp {
+
+static bool dtype_ok(int dtype) { return dtype == SVDMLP_BF16 || dtype == SVDMLP_F16; }
+
+// Base and strides (elements of 2 bytes) on 16-byte boundaries.
+static bool rows_aligned(const void* p, int64_t token, int64_t head) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && token % 8 == 0 && head % 8 == 0;
+}
+
+static bool elems_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+// --------------------------------------------------------------------- rope
+template <typename T, int E>
+static int launch_rope(const RopeParams& p, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((p.tokens + p.tile - 1) / p.tile);
+  rope_kernel<T, E><<<grid, kRopeThreads, static_cast<size_t>(p.tile) * p.half * sizeof(float2), s>>>(p);
+  SVD_CUDA(cudaGetLastError());
+  count_launch();
+  return SVDMLP_OK;
+}
+
+static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
+  if (!a || !a->q || !a->k || !a->positions || !a->inv_freq || !a->q_out) return SVDMLP_ERR_INVALID_VALUE;
+  if (a->tokens <= 0 || a->q_heads <= 0 || a->kv_heads <= 0 || a->head_dim <= 0) return SVDMLP_ERR_INVALID_VALUE;
+  if (!dtype_ok(a->dtype)) return SVDMLP_ERR_DTYPE;
+  if (a->rotary_dim <= 0 || a->rotary_dim % 2 != 0 || a->rotary_dim > a->head_dim || a->head_dim > 512)
+    return SVDMLP_ERR_SHAPE_MISMATCH;
+  if (!std::isfinite(a->scale)) return SVDMLP_ERR_INVALID_VALUE;
+  if ((a->k_cache == nullptr) != (a->v_cache == nullptr)) return SVDMLP_ERR_INVALID_VALUE;
+  const bool cached = a->k_cache != nullptr;
+  if (!cached && !a->k_out) return SVDMLP_ERR_INVALID_VALUE;
+  if (cached && (!a->v || !a->slots || a->block_size <= 0 || a->num_blocks <= 0)) return SVDMLP_ERR_INVALID_VALUE;
+  if (cached) {
+    const int64_t inside = static_cast<int64_t>(a->kv_heads) * a->block_size * a->head_dim;
+    if (a->k_block < inside || a->v_block < inside) return SVDMLP_ERR_SHAPE_MISMATCH;
+  }
+  RopeParams p{};
+  p.tokens = a->tokens;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  p.half = a->rotary_dim / 2;
+  p.interleaved = a->interleaved != 0;
+  p.block_size = a->block_size;
+  p.block_shift = -1;
+  if (cached && (a->block_size & (a->block_size - 1)) == 0)
+    for (p.block_shift = 0; (1 << p.block_shift) < a->block_size;) ++p.block_shift;
+  p.scale = a->scale;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.q_token = a->q_token;
+  p.q_head = a->q_head;
+  p.k_token = a->k_token;
+  p.k_head = a->k_head;
+  p.v_token = a->v_token;
+  p.v_head = a->v_head;
+  p.positions = a->positions;
+  p.slots = reinterpret_cast<const long long*>(a->slots);
+  p.inv_freq = a->inv_freq;
+  p.q_out = a->q_out;
+  p.k_out = a->k_out;
+  p.k_cache = a->k_cache;
+  p.v_cache = a->v_cache;
+  p.k_block = a->k_block;
+  p.v_block = a->v_block;
+  p.cache_slots = static_cast<long long>(a->block_size) * a->num_blocks;
+  p.tile = std::max(1, std::min(kRopeMaxTile, a->tokens / (4 * planning_sms())));
+  bool vec = p.half % 8 == 0 && p.head_dim % 8 == 0 && rows_aligned(p.q, p.q_token, p.q_head) &&
+             rows_aligned(p.k, p.k_token, p.k_head) && rows_aligned(p.q_out, 0, 0) && rows_aligned(p.k_out, 0, 0);
+  if (cached)
+    vec = vec && rows_aligned(p.v, p.v_token, p.v_head) && rows_aligned(p.k_cache, p.k_block, 0) &&
+          rows_aligned(p.v_cache, p.v_block, 0);
+  if (!elems_aligned(p.q) || !elems_aligned(p.k) || !elems_aligned(p.v) || !elems_aligned(p.q_out) ||
+      !elems_aligned(p.k_out) || !elems_aligned(p.k_cache) || !elems_aligned(p.v_cache))
+    return SVDMLP_ERR_ALIGNMENT;
+  if (a->dtype == SVDMLP_BF16)
+    return vec ? launch_rope<__nv_bfloat16, 8>(p, s) : launch_rope<__nv_bfloat16, 1>(p, s);
+  return vec ? launch_rope<__half, 8>(p, s) : launch_rope<__half, 1>(p, s);
+}
+
+// -------------------------------------------------------------------- pages
+static int pages_impl(const svdmlp_pages_args* a, cudaStream_t s) {
+  if (!a || !a->table || !a->held || !a->added || !a->free_count || !a->cu || !a->lens || !a->count_out || !a->missing)
+    return SVDMLP_ERR_INVALID_VALUE;
+  if (a->batch <= 0 || a->tokens < 0 || a->block_size <= 0 || a->table_width <= 0 || a->free_capacity < 0)
+    return SVDMLP_ERR_INVALID_VALUE;
+  if (a->ld_table < a->table_width) return SVDMLP_ERR_SHAPE_MISMATCH;
+  if ((a->tokens > 0 && (!a->slots || !a->positions)) || (a->free_capacity > 0 && !a->free_blocks))
+    return SVDMLP_ERR_INVALID_VALUE;
+  PagesParams p{};
+  p.batch = a->batch;
+  p.tokens = a->tokens;
+  p.block_size = a->block_size;
+  p.width = a->table_width;
+  p.capacity = a->free_capacity;
+  p.table = a->table;
+  p.ld_table = a->ld_table;
+  p.held = a->held;
+  p.added = a->added;
+  p.free_blocks = a->free_blocks;
+  p.free_count = a->free_count;
+  p.slots = reinterpret_cast<long long*>(a->slots);
+  p.positions = a->positions;
+  p.cu = a->cu;
+  p.lens = a->lens;
+  p.count_out = a->count_out;
+  p.missing = a->missing;
+  const int grid = std::max(1, std::min(planning_sms(), (a->tokens + kPagesThreads - 1) / kPagesThreads));
+  page_step_kernel<<<static_cast<unsigned>(grid), kPagesThreads, 0, s>>>(p);
+  SVD_CUDA(cudaGetLastError());
+  count_launch();
+  return SVDMLP_OK;
+}
+
+// ---------------------------------------------------------------- attention
+static int check_heads(int dtype, int q_heads, int kv_heads, int head_dim, float scale) {
+  if (q_heads <= 0 || kv_heads <= 0) return SVDMLP_ERR_INVALID_VALUE;
+  if (!dtype_ok(dtype)) return SVDMLP_ERR_DTYPE;
+  if (q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128)) return SVDMLP_ERR_SHAPE_MISMATCH;
+  if (!std::isfinite(scale)) return SVDMLP_ERR_INVALID_VALUE;
+  return SVDMLP_OK;
+}
+
+static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
+  if (!a || !a->q || !a->k || !a->v || !a->cu_q || !a->cu_k || !a->out) return SVDMLP_ERR_INVALID_VALUE;
+  if (a->batch <= 0 || a->q_tokens <= 0 || a->k_tokens <= 0) return SVDMLP_ERR_INVALID_VALUE;
+  SVD_CHECK(check_heads(a->dtype, a->q_heads, a->kv_heads, a->head_dim, a->scale));
+  if (!rows_aligned(a->q, a->q_token, a->q_head) || !rows_aligned(a->k, a->k_token, a->k_head) ||
+      !rows_aligned(a->v, a->v_token, a->v_head) || !rows_aligned(a->out, a->out_token, a->out_head))
+    return SVDMLP_ERR_ALIGNMENT;
+  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return SVDMLP_ERR_INVALID_VALUE;
+  if (a->workspace_bytes < svdmlp_prompt_workspace_bytes()) return SVDMLP_ERR_WORKSPACE;
+  const long long warps = static_cast<long long>(a->q_tokens) * a->q_heads;
+  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
+  if (a->dtype == SVDMLP_BF16) {
+    if (a->head_dim == 128) prompt_rows_kernel<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(*a);
+    else prompt_rows_kernel<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(*a);
+  } else {
+    if (a->head_dim == 128) prompt_rows_kernel<__half, 128><<<grid, 256, 0, s>>>(*a);
+    else prompt_rows_kernel<__half, 64><<<grid, 256, 0, s>>>(*a);
+  }
+  SVD_CUDA(cudaGetLastError());
+  count_launch();
+  return SVDMLP_OK;
+}
+
+static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
+  if (!a || !a->q || !a->k_cache || !a->v_cache || !a->table || !a->lens || !a->cu_q || !a->out)
+    return SVDMLP_ERR_INVALID_VALUE;
+  if (a->batch <= 0 || a->tokens <= 0 || a->num_blocks <= 0 || a->table_width <= 0 || a->max_tree <= 0)
+    return SVDMLP_ERR_INVALID_VALUE;
+  SVD_CHECK(check_heads(a->dtype, a->q_heads, a->kv_heads, a->head_dim, a->scale));
+  if (a->block_size < 8 || a->block_size > 1024 || (a->block_size & (a->block_size - 1)) != 0)
+    return SVDMLP_ERR_SHAPE_MISMATCH;
+  const int64_t inside = static_cast<int64_t>(a->kv_heads) * a->block_size * a->head_dim;
+  if (a->k_block < inside || a->v_block < inside || a->ld_table < a->table_width) return SVDMLP_ERR_SHAPE_MISMATCH;
+  if (!rows_aligned(a->q, a->q_token, a->q_head) || !rows_aligned(a->k_cache, a->k_block, 0) ||
+      !rows_aligned(a->v_cache, a->v_block, 0) || !rows_aligned(a->out, a->out_token, a->out_head))
+    return SVDMLP_ERR_ALIGNMENT;
+  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return SVDMLP_ERR_INVALID_VALUE;
+  if (a->workspace_bytes < svdmlp_tree_workspace_bytes(a->head_dim)) return SVDMLP_ERR_WORKSPACE;
+  const long long warps = static_cast<long long>(a->tokens) * a->q_heads;
+  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
+  if (a->dtype == SVDMLP_BF16) {
+    if (a->head_dim == 128) tree_rows_kernel<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(*a);
+    else tree_rows_kernel<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(*a);
+  } else {
+    if (a->head_dim == 128) tree_rows_kernel<__half, 128><<<grid, 256, 0, s>>>(*a);
+    else tree_rows_kernel<__half, 64><<<grid, 256, 0, s>>>(*a);
+  }
+  SVD_CUDA(cudaGetLastError());
+  count_launch();
+  return SVDMLP_OK;
+}
+
+}  // namespace svdmlp
+
+extern "C" {
+
+int svdmlp_rope(const svdmlp_rope_args* args, void* stream) {
+  return svdmlp::rope_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+int svdmlp_page_step(const svdmlp_pages_args* args, void* stream) {
+  return svdmlp::pages_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+int64_t svdmlp_prompt_workspace_bytes(void) { return 256; }
+
+int svdmlp_prompt_attention(const svdmlp_prompt_args* args, void* stream) {
+  return svdmlp::prompt_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+int64_t svdmlp_tree_workspace_bytes(int32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return SVDMLP_ERR_SHAPE_MISMATCH;
+  return 256;
+}
+
+int svdmlp_tree_attention(const svdmlp_tree_args* args, void* stream) {
+  return svdmlp::tree_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

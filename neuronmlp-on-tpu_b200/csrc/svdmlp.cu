@@ -19,6 +19,7 @@
 #include "../../include/svdmlp.h"
 #include "gemm_sm100.cuh"
 #include "gemv_sm100.cuh"
+#include "host.h"
 #include "layer_decode_sm100.cuh"
 #include "peer_sm100.cuh"
 
@@ -68,20 +69,12 @@ static bool g_timing = false;
 static std::vector<TimedLaunch> g_timed;
 static size_t g_timed_used = 0;
 
-static int cuda_fail(cudaError_t e) {
+int cuda_fail(cudaError_t e) {
   g_last_cuda_error = static_cast<int>(e);
   return SVDMLP_ERR_CUDA;
 }
-#define SVD_CUDA(call)                         \
-  do {                                         \
-    cudaError_t e_ = (call);                   \
-    if (e_ != cudaSuccess) return cuda_fail(e_); \
-  } while (0)
-#define SVD_CHECK(...)      \
-  do {                      \
-    int s_ = (__VA_ARGS__); \
-    if (s_ != SVDMLP_OK) return s_; \
-  } while (0)
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+unsigned long long wait_limit_ns() { return g_wait_limit_ns; }
 
 static int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -93,6 +86,14 @@ struct DeviceInfo {
 };
 static std::mutex g_dev_mu;
 static DeviceInfo g_dev[64];
+
+static int device_info(DeviceInfo** out);
+int device_sms(int* sms) {
+  DeviceInfo* d = nullptr;
+  SVD_CHECK(device_info(&d));
+  *sms = d->sms;
+  return SVDMLP_OK;
+}
 
 static int device_info(DeviceInfo** out) {
   int dev = 0;
@@ -111,7 +112,7 @@ static int device_info(DeviceInfo** out) {
 
 // Number of SMs used for planning: the current device's, or 148 (B200) when
 // no device is visible (workspace sizing on a host without a GPU).
-static int planning_sms() {
+int planning_sms() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) == cudaSuccess &&
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && sms > 0)
@@ -121,7 +122,7 @@ static int planning_sms() {
 }
 
 // ------------------------------------------------------------- tensor maps
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {

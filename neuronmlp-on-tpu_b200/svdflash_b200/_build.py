@@ -15,13 +15,13 @@ PKG_DIR = pathlib.Path(__file__).resolve().parent
 CSRC = PKG_DIR.parent / "csrc"
 INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "_native" / "libsvdmlp.so"
-SOURCES = [CSRC / "svdmlp.cu"]
-HEADERS = [*sorted(CSRC.glob("*.cuh")), INCLUDE / "svdmlp.h"]
+SOURCES = [CSRC / "svdmlp.cu", CSRC / "attention.cu"]
+HEADERS = [*sorted(CSRC.glob("*.cuh")), CSRC / "host.h", INCLUDE / "svdmlp.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "--threads", "0",
 ]
 
 

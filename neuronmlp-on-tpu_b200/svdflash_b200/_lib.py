@@ -6,6 +6,7 @@ If the shared library is missing the import fails loudly.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
@@ -53,6 +54,38 @@ class Layout(ctypes.Structure):
         ("packed_bytes", c_int64),
     ]
 
+
+BF16 = 0
+F16 = 1
+
+
+def _args(name: str, *groups):
+    """An argument struct of the C ABI: (its ctypes mirror, a function that
+    packs its fields, in order, into bytes).  A call passes the bytes: filling
+    a ctypes structure field by field would cost several times as much."""
+    kinds = {"i": c_int32, "f": c_float, "p": c_void_p, "q": c_int64}
+    fields = [(n, kinds[k]) for k, names in groups for n in names.split()]
+    packer = struct.Struct("@" + "".join(k.upper() if k == "p" else k for k, names in groups for _ in names.split()))
+    mirror = type(name, (ctypes.Structure,), {"_fields_": fields})
+    return mirror, packer.pack
+
+
+RopeArgs, ROPE_ARGS = _args(
+    "RopeArgs", ("i", "dtype tokens q_heads kv_heads head_dim rotary_dim interleaved block_size num_blocks"),
+    ("f", "scale"), ("p", "q k v"), ("q", "q_token q_head k_token k_head v_token v_head"),
+    ("p", "positions slots inv_freq q_out k_out k_cache v_cache"), ("q", "k_block v_block"))
+PagesArgs, PAGES_ARGS = _args(
+    "PagesArgs", ("i", "batch tokens block_size table_width free_capacity reserved"), ("p", "table"),
+    ("q", "ld_table"), ("p", "held added free_blocks free_count slots positions cu lens count_out missing"))
+PromptArgs, PROMPT_ARGS = _args(
+    "PromptArgs", ("i", "dtype batch q_tokens k_tokens q_heads kv_heads head_dim causal"), ("f", "scale"),
+    ("i", "reserved"), ("p", "q k v"), ("q", "q_token q_head k_token k_head v_token v_head"), ("p", "cu_q cu_k out"),
+    ("q", "out_token out_head"), ("p", "workspace"), ("q", "workspace_bytes"))
+TreeArgs, TREE_ARGS = _args(
+    "TreeArgs", ("i", "dtype batch tokens q_heads kv_heads head_dim block_size num_blocks table_width max_tree"),
+    ("f", "scale"), ("i", "reserved"), ("p", "q"), ("q", "q_token q_head"), ("p", "k_cache v_cache"),
+    ("q", "k_block v_block"), ("p", "table"), ("q", "ld_table"), ("p", "lens cu_q mask out"),
+    ("q", "out_token out_head"), ("p", "workspace"), ("q", "workspace_bytes"))
 
 LP = POINTER(Layout)
 V = c_void_p
@@ -123,6 +156,12 @@ SIGNATURES = {
                                                 c_int, c_int64, V, I64, V]),
     "svdmlp_peer_sum_f16": (c_int, [POINTER(c_void_p), c_int, c_int, c_int64, c_int, c_int, c_int, c_int64,
                                     c_void_p, c_int64, c_void_p]),
+    "svdmlp_rope": (c_int, [V, V]),
+    "svdmlp_page_step": (c_int, [V, V]),
+    "svdmlp_prompt_workspace_bytes": (c_int64, []),
+    "svdmlp_prompt_attention": (c_int, [V, V]),
+    "svdmlp_tree_workspace_bytes": (c_int64, [c_int32]),
+    "svdmlp_tree_attention": (c_int, [V, V]),
 }
 
 _lock = threading.Lock()

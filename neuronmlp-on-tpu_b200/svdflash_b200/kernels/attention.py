@@ -1,0 +1,425 @@
+"""The attention half of a decoder layer on the B200 kernels.
+
+The reference runs its MLP inside a LLaMA decoder layer (models/modeling_llama.py:
+rotary positions, KV cache, grouped-query attention; bench/e2e_block.py:208-229
+for the prefill block).  These are its operators here, for serving:
+
+* ``rope_cache`` / ``rope``: rotary positions, with the keys and values written
+  into a paged cache in the same pass; ``rope_frequencies`` gives the tables of
+  contexts stretched beyond the trained length;
+* ``prompt_attention``: causal attention over packed prompts;
+* ``tree_attention``: attention of each request's newest tokens (one token, a
+  chain, or a tree of drafted tokens) over the paged cache;
+* ``page_step``: block tables, slots and positions from request lengths, on the
+  GPU.
+
+Tensors are CUDA tensors, activations bf16 or fp16 ``[tokens, heads, head_dim]``
+with any token and head strides (views of one q|k|v projection are read in
+place).  A layer's cache is two tensors ``[num_blocks, kv_heads, block_size,
+head_dim]``.  Softmax statistics and sums are fp32.  The work goes to the
+current stream of the tensors' device and nothing synchronises, so a step can
+be captured in a CUDA graph.  There is no CPU path and no backward (the library
+is for inference).
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from .. import _lib
+from . import ops
+
+__all__ = ["PageStep", "kv_cache", "page_step", "prompt_attention", "rope", "rope_cache", "rope_frequencies",
+           "tree_attention"]
+
+_DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+# -------------------------------------------------------------------- checks
+def _dtype(t: torch.Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"supported dtypes are bfloat16 and float16, got {t.dtype}")
+    return code
+
+
+def _heads(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A [tokens, heads, head_dim] CUDA tensor, of the type, device and head size of `like`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if t.dim() != 3 or t.shape[1] <= 0 or t.shape[2] <= 0:
+        raise ValueError(f"{name}: expected [tokens, heads, head_dim], got {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the B200 path has no CPU fallback)")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError("all inputs must have the same dtype")
+        if t.device != like.device:
+            raise ValueError("inputs must be CUDA tensors on one device")
+        if t.shape[2] != like.shape[2]:
+            raise ValueError(f"{name} has head_dim {t.shape[2]}, expected {like.shape[2]}: dimensions do not match")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _vector_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a copy of it when its rows do not lie on 16-byte boundaries."""
+    if t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}: dimensions do not match")
+    if t.device != device:
+        raise ValueError("inputs must be CUDA tensors on one device")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _offsets(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor")
+    if t.dim() != 1 or t.shape[0] < 2:
+        raise ValueError(f"{name} must be [batch + 1], got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError("inputs must be CUDA tensors on one device")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv_heads: Optional[int]):
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+        if t.dim() != 4 or min(t.shape) <= 0:
+            raise ValueError(f"{name}: expected [num_blocks, kv_heads, block_size, head_dim], got {tuple(t.shape)}")
+        if t.dtype != like.dtype:
+            raise TypeError("all inputs must have the same dtype")
+        if t.device != like.device:
+            raise ValueError("inputs must be CUDA tensors on one device")
+        if t.shape[3] != like.shape[2] or (kv_heads is not None and t.shape[1] != kv_heads):
+            raise ValueError(f"{name} {tuple(t.shape)} does not match the heads: dimensions do not match")
+        d, b = t.shape[3], t.shape[2]
+        if t.stride(3) != 1 or t.stride(2) != d or t.stride(1) != b * d:
+            raise ValueError(f"{name} must be contiguous inside a block")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have matching shapes")
+
+
+def _scale(scale: Optional[float], head_dim: int) -> float:
+    if scale is None:
+        return 1.0 / math.sqrt(head_dim)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return float(scale)
+
+
+def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if tuple(out.shape) != tuple(q.shape) or out.device != q.device:
+        raise ValueError(f"out must be {tuple(q.shape)} on {q.device}: dimensions do not match")
+    if out.dtype != q.dtype:
+        raise TypeError("out must have the inputs' dtype")
+    if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+        raise ValueError("out must have 16-byte aligned rows")
+    return out
+
+
+def _call(fn, args: bytes, device: torch.device, what: str) -> None:
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        _lib.check(status, what)
+
+
+# -------------------------------------------------------------------- rotary
+def rope_frequencies(head_dim: int, *, base: float = 10000.0, rotary_dim: Optional[int] = None,
+                     scaling: Optional[dict] = None, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(inv_freq [rotary_dim / 2] fp32, scale) of rotary positions.
+
+    `scaling` stretches the context, with a checkpoint's own keys
+    (``rope_type`` or ``type``):
+
+    * ``linear``: every frequency divided by ``factor``;
+    * ``llama3``: frequencies whose wavelength exceeds
+      ``original_max_position_embeddings / low_freq_factor`` divided by
+      ``factor``, those below ``original / high_freq_factor`` kept, a linear
+      blend of the two between;
+    * ``yarn``: the same between the pairs that turn ``beta_fast`` (32) and
+      ``beta_slow`` (1) times over the original context, linear in the pair's
+      index, and a magnitude of 0.1 ln(factor) + 1 (``attention_factor``
+      overrides it).
+    """
+    rot = head_dim if rotary_dim is None else rotary_dim
+    if isinstance(rot, bool) or not isinstance(rot, int) or rot <= 0 or rot % 2 or rot > head_dim:
+        raise ValueError(f"rotary_dim must be a positive even integer of at most head_dim, got {rot}")
+    if not base > 0:
+        raise ValueError(f"base must be positive, got {base}")
+    half = rot // 2
+    freq = [base ** (-i / half) for i in range(half)]
+    magnitude = 1.0
+    kind = "default" if not scaling else scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "linear":
+        freq = [f / scaling["factor"] for f in freq]
+    elif kind == "llama3":
+        factor, context = scaling["factor"], scaling["original_max_position_embeddings"]
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        if high <= low:
+            raise ValueError("high_freq_factor must exceed low_freq_factor")
+        turns = [f * context / (2 * math.pi) for f in freq]
+        keep = [min(1.0, max(0.0, (t - low) / (high - low))) for t in turns]
+        freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
+    elif kind == "yarn":
+        factor, context = scaling["factor"], scaling["original_max_position_embeddings"]
+
+        def pair_that_turns(times):
+            return half * math.log(context / (2 * math.pi * times)) / math.log(base)
+
+        first = max(math.floor(pair_that_turns(scaling.get("beta_fast", 32))), 0)
+        last = min(math.ceil(pair_that_turns(scaling.get("beta_slow", 1))), rot - 1)
+        span = max(last - first, 0.001)
+        keep = [1 - min(1.0, max(0.0, (i - first) / span)) for i in range(half)]
+        freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
+        magnitude = scaling.get("attention_factor") or (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+    elif kind != "default":
+        raise ValueError(f"unknown rotary scaling {kind!r} (default, linear, llama3, yarn)")
+    return torch.tensor(freq, dtype=torch.float32, device=device), float(magnitude)
+
+
+def _rope(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, scale, return_k):
+    q = _heads("q", q)
+    code = _dtype(q)
+    k = _heads("k", k, q)
+    n, h, d = q.shape
+    hk = k.shape[1]
+    device = q.device
+    if k.shape[0] != n:
+        raise ValueError("q and k must have the same tokens: dimensions do not match")
+    positions = _index("positions", positions, torch.int32, (n,), device)
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32:
+        raise TypeError("inv_freq must be a float32 tensor")
+    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be [rotary_dim / 2] with rotary_dim at most {d}, got {tuple(inv_freq.shape)}")
+    if inv_freq.device != device:
+        raise ValueError("inputs must be CUDA tensors on one device")
+    vs = slots_ptr = kc = vc = kb = vb = bs = nb = 0
+    v_strides = (0, 0)
+    if k_cache is not None:
+        v = _heads("v", v, q)
+        if v.shape != k.shape:
+            raise ValueError("k and v must have matching shapes")
+        slots = _index("slots", slots, torch.int64, (n,), device)
+        _caches(k_cache, v_cache, q, hk)
+        vs, slots_ptr, v_strides = v.data_ptr(), slots.data_ptr(), v.stride()
+        kc, vc, kb, vb = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), v_cache.stride(0)
+        nb, bs = k_cache.shape[0], k_cache.shape[2]
+    q_out = torch.empty((n, h, d), dtype=q.dtype, device=device)
+    k_out = torch.empty((n, hk, d), dtype=q.dtype, device=device) if return_k else None
+    if n == 0:
+        return q_out, k_out
+    args = _lib.ROPE_ARGS(code, n, h, hk, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, bs, nb, scale,
+                          q.data_ptr(), k.data_ptr(), vs, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                          v_strides[0], v_strides[1], positions.data_ptr(), slots_ptr, inv_freq.data_ptr(),
+                          q_out.data_ptr(), k_out.data_ptr() if return_k else 0, kc, vc, kb, vb)
+    _call(_lib.load().svdmlp_rope, args, device, "rope")
+    return q_out, k_out
+
+
+def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+               inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, interleaved: bool = False,
+               scale: float = 1.0, return_k: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotates q [N, Hq, D] and k [N, Hk, D] to `positions` (int32 [N]) and
+    writes the rotated k, and v, into the paged cache at `slots` (int64 [N];
+    page_step gives both).  Returns (q, k), k only with `return_k`.
+
+    The first 2 * len(inv_freq) elements of a head turn: pairs (i, i + half), or
+    neighbours when `interleaved`; `scale` multiplies what turns.  A token whose
+    slot is negative is written nowhere; two tokens of one call must not share a
+    slot."""
+    return _rope(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, scale, return_k)
+
+
+def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+         interleaved: bool = False, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """rope_cache without a cache: returns the rotated (q, k)."""
+    return _rope(q, k, None, positions, None, inv_freq, None, None, interleaved, scale, True)
+
+
+# -------------------------------------------------------------------- paging
+class PageStep(NamedTuple):
+    slots: torch.Tensor        # int64 [num_tokens]: where each new token goes, -1: nowhere
+    positions: torch.Tensor    # int32 [num_tokens]: its position in its request
+    cu_seqlens: torch.Tensor   # int32 [batch + 1]: offsets of the requests' new tokens
+    seq_lens: torch.Tensor     # int32 [batch]: tokens held after this step
+    free_count: torch.Tensor   # int32 [1]: blocks left on the free list
+    missing: torch.Tensor      # int32 [1]: blocks the free list could not give
+
+
+def kv_cache(num_blocks: int, kv_heads: int, block_size: int, head_dim: int, *, dtype=torch.bfloat16,
+             device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k_cache, v_cache) of one layer, zeroed: [num_blocks, kv_heads, block_size, head_dim]."""
+    for name, value in (("num_blocks", num_blocks), ("kv_heads", kv_heads), ("block_size", block_size),
+                        ("head_dim", head_dim)):
+        ops._positive(name, value)
+    both = torch.zeros((2, num_blocks, kv_heads, block_size, head_dim), dtype=dtype, device=device)
+    return both[0], both[1]
+
+
+def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks: torch.Tensor,
+              free_count: torch.Tensor, block_size: int, num_tokens: int) -> PageStep:
+    """Block tables, slots and positions of one forward pass from request lengths.
+
+    Request b holds seq_lens[b] tokens and adds new_lens[b] (int32 [B]).  The
+    blocks that it lacks come off the end of free_blocks[:free_count] (int32
+    [F], int32 [1]), requests in order, and are entered into block_table [B, W]
+    in place.  `num_tokens`, known to the caller, is at least the sum of
+    new_lens; entries beyond it get slot -1.  The inputs other than
+    block_table are left as they are: a caller keeps the returned seq_lens and
+    free_count for the next step, and frees blocks by writing them behind
+    free_count.  `missing` above zero means that the free list ran out: those
+    blocks' entries and slots are -1."""
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.dim() != 2 or min(block_table.shape) <= 0 or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be a nonempty row-major [batch, width], got {tuple(block_table.shape)}")
+    if not block_table.is_cuda:
+        raise ValueError("block_table must be a CUDA tensor (the B200 path has no CPU fallback)")
+    device = block_table.device
+    b, width = block_table.shape
+    seq_lens = _index("seq_lens", seq_lens, torch.int32, (b,), device)
+    new_lens = _index("new_lens", new_lens, torch.int32, (b,), device)
+    free_count = _index("free_count", free_count, torch.int32, (1,), device)
+    if not isinstance(free_blocks, torch.Tensor) or free_blocks.dtype != torch.int32:
+        raise TypeError("free_blocks must be an int32 tensor")
+    if free_blocks.dim() != 1 or not free_blocks.is_contiguous() or free_blocks.device != device:
+        raise ValueError("free_blocks must be a contiguous 1D tensor on the table's device")
+    ops._positive("block_size", block_size)
+    if isinstance(num_tokens, bool) or not isinstance(num_tokens, int) or num_tokens < 0:
+        raise ValueError(f"num_tokens must be a nonnegative integer, got {num_tokens}")
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=device)
+    whole = torch.empty(num_tokens + 2 * b + 3, dtype=torch.int32, device=device)
+    at = whole.data_ptr()
+    positions, cu, lens, left, missing = whole.split((num_tokens, b + 1, b, 1, 1))
+    cu_at = at + 4 * num_tokens
+    lens_at = cu_at + 4 * (b + 1)
+    left_at = lens_at + 4 * b
+    args = _lib.PAGES_ARGS(b, num_tokens, block_size, width, free_blocks.shape[0], 0, block_table.data_ptr(),
+                           block_table.stride(0), seq_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
+                           free_count.data_ptr(), slots.data_ptr(), at, cu_at, lens_at, left_at, left_at + 4)
+    _call(_lib.load().svdmlp_page_step, args, device, "page_step")
+    return PageStep(slots, positions, cu, lens, left, missing)
+
+
+# ----------------------------------------------------------------- attention
+def _group(q: torch.Tensor, kv_heads: int) -> None:
+    if q.shape[1] % kv_heads:
+        raise ValueError(f"{q.shape[1]} query heads are no multiple of {kv_heads} key/value heads")
+    if q.shape[2] not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {q.shape[2]}")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: Optional[torch.Tensor] = None, *, causal: bool = True, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over packed sequences: q [Nq, Hq, D], k and v
+    [Nk, Hk, D], sequence b the rows cu_q[b] .. cu_q[b + 1] and the keys cu_k[b]
+    .. cu_k[b + 1] (int32 [B + 1] on the device; cu_k defaults to cu_q).  When
+    causal, the queries are the last tokens of their sequence: query i of n
+    sees the first m - n + i + 1 of m keys.  Rows that see no key, and rows of
+    no sequence, give zeros.  `scale` defaults to 1 / sqrt(D).  bf16 or fp16,
+    D 64 or 128; the probabilities are rounded to the inputs' type for the
+    product with v, statistics and sums are fp32."""
+    q = _heads("q", q)
+    code = _dtype(q)
+    k, v = _heads("k", k, q), _heads("v", v, q)
+    if k.shape != v.shape:
+        raise ValueError("k and v must have matching shapes")
+    nq, h, d = q.shape
+    nk, hk = k.shape[0], k.shape[1]
+    _group(q, hk)
+    device = q.device
+    cu_q = _offsets("cu_q", cu_q, device)
+    if cu_k is None:
+        if nq != nk:
+            raise ValueError("without cu_k, q and k must have the same tokens: dimensions do not match")
+        cu_k = cu_q
+    else:
+        cu_k = _offsets("cu_k", cu_k, device)
+        if cu_k.shape != cu_q.shape:
+            raise ValueError("cu_q and cu_k must have matching shapes")
+    scale = _scale(scale, d)
+    out = _output(out, q)
+    if nq == 0:
+        return out
+    if nk == 0:
+        return out.zero_()
+    q, k, v = _vector_rows(q), _vector_rows(k), _vector_rows(v)
+    lib = _lib.load()
+    ws = ops.workspace_for(device, lib.svdmlp_prompt_workspace_bytes())
+    args = _lib.PROMPT_ARGS(code, cu_q.shape[0] - 1, nq, nk, h, hk, d, 1 if causal else 0, scale, 0, q.data_ptr(),
+                            k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                            v.stride(0), v.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), out.stride(0),
+                            out.stride(1), ws.ptr, ws.nbytes)
+    _call(lib.svdmlp_prompt_attention, args, device, "prompt_attention")
+    return out
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, cu_q: torch.Tensor, *, max_tree: int,
+                   tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of each request's newest tokens over the paged cache, which
+    already holds their keys and values (rope_cache wrote them).
+
+    q [N, Hq, D]; request b has the rows cu_q[b] .. cu_q[b + 1] (int32 [B + 1]),
+    n of them, and seq_lens[b] tokens (int32 [B]) in the blocks block_table[b]
+    names (int32 [B, W]); the newest n are its tree, in the rows' order.  Every
+    row sees the seq_lens[b] - n tokens of the context.  In the tree, row i sees
+    token j when bit j of tree_mask[row] (int64 [N]: a token's ancestors and
+    itself, up to 64) is set; without a mask, when j <= i, so n = 1 is ordinary
+    decoding and a chain needs no mask.  `max_tree` is the largest n expected
+    (it sizes the tiles; larger trees are still computed).  Rows that see
+    nothing give zeros.  The block size is a power of two from 8 to 1024."""
+    q = _heads("q", q)
+    code = _dtype(q)
+    _caches(k_cache, v_cache, q, None)
+    n, h, d = q.shape
+    hk, bs = k_cache.shape[1], k_cache.shape[2]
+    _group(q, hk)
+    if bs & (bs - 1) or not 8 <= bs <= 1024:
+        raise ValueError(f"the cache's block size must be a power of two from 8 to 1024, got {bs}")
+    device = q.device
+    cu_q = _offsets("cu_q", cu_q, device)
+    b = cu_q.shape[0] - 1
+    seq_lens = _index("seq_lens", seq_lens, torch.int32, (b,), device)
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.dim() != 2 or block_table.shape[0] != b or block_table.shape[1] <= 0 or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be row-major [{b}, width], got {tuple(block_table.shape)}: "
+                         "dimensions do not match")
+    if block_table.device != device:
+        raise ValueError("inputs must be CUDA tensors on one device")
+    if tree_mask is not None:
+        tree_mask = _index("tree_mask", tree_mask, torch.int64, (n,), device)
+    ops._positive("max_tree", max_tree)
+    scale = _scale(scale, d)
+    out = _output(out, q)
+    if n == 0:
+        return out
+    q = _vector_rows(q)
+    lib = _lib.load()
+    ws = ops.workspace_for(device, lib.svdmlp_tree_workspace_bytes(d))
+    args = _lib.TREE_ARGS(code, b, n, h, hk, d, bs, k_cache.shape[0], block_table.shape[1], max_tree, scale, 0,
+                          q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+                          k_cache.stride(0), v_cache.stride(0), block_table.data_ptr(), block_table.stride(0),
+                          seq_lens.data_ptr(), cu_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
+                          out.data_ptr(), out.stride(0), out.stride(1), ws.ptr, ws.nbytes)
+    _call(lib.svdmlp_tree_attention, args, device, "tree_attention")
+    return out
