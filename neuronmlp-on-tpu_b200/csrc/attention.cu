@@ -5,11 +5,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
 #include "../../include/svdmlp.h"
-#include "attention_rows.cuh"
+#include "attention_sm100.cuh"
 #include "host.h"
 #include "rope_pages.cuh"
 
@@ -137,6 +138,104 @@ static int check_heads(int dtype, int q_heads, int kv_heads, int head_dim, float
   return SVDMLP_OK;
 }
 
+// ------------------------------------------------------------- tensor maps
+static int attn_map(CUtensorMap* map, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides,
+                    const int* box) {
+  auto fn = encode_fn();
+  if (!fn) return cuda_fail(cudaErrorInitializationError);
+  cuuint64_t d[5], st[5];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+    if (i > 0) st[i - 1] = static_cast<cuuint64_t>(strides[i] * 2);
+  }
+  const CUresult r =
+      fn(map, dtype == SVDMLP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+         static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SVDMLP_OK : SVDMLP_ERR_ALIGNMENT;
+}
+
+// The query heads that share a key/value head lie in one tile, up to 64 of them.
+static int pack_of(int group) { return group <= 64 ? group : 1; }
+
+static int query_map(CUtensorMap* map, int dtype, const void* q, int tokens, int q_heads, int head_dim, int gp,
+                     int64_t token, int64_t head) {
+  const int64_t dims[4] = {head_dim, gp, q_heads / gp, tokens}, strides[4] = {1, head, head * gp, token};
+  const int box[4] = {64, gp, 1, 128 / gp};
+  return attn_map(map, dtype, q, 4, dims, strides, box);
+}
+
+// ------------------------------------------------------------------- launch
+static constexpr int64_t kAttnCtlBytes = 256, kAttnCounterBytes = 1 << 20;  // as svdmlp_workspace_init lays them out
+
+template <int D>
+static int64_t attn_workspace() {
+  return kAttnCtlBytes + kAttnCounterBytes +
+         static_cast<int64_t>(std::min(planning_sms(), kAttnMaxGrid)) * 2 * AttnCfg<D>::PART_FLOATS * 4;
+}
+
+template <typename T, int D, bool PAGED>
+static int launch_attention(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnParams& p,
+                            int grid, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
+  int dev = 0;
+  SVD_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    SVD_CUDA(cudaFuncSetAttribute(attention_kernel<T, D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  AttnCfg<D>::SMEM_BYTES));
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  attention_kernel<T, D, PAGED><<<static_cast<unsigned>(grid), kAttnThreads, AttnCfg<D>::SMEM_BYTES, s>>>(q, k, v, p);
+  SVD_CUDA(cudaGetLastError());
+  count_launch();
+  return SVDMLP_OK;
+}
+
+template <bool PAGED>
+static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                              const AttnParams& p, int grid, cudaStream_t s) {
+  if (dtype == SVDMLP_BF16)
+    return head_dim == 128 ? launch_attention<__nv_bfloat16, 128, PAGED>(q, k, v, p, grid, s)
+                           : launch_attention<__nv_bfloat16, 64, PAGED>(q, k, v, p, grid, s);
+  return head_dim == 128 ? launch_attention<__half, 128, PAGED>(q, k, v, p, grid, s)
+                         : launch_attention<__half, 64, PAGED>(q, k, v, p, grid, s);
+}
+
+// What both attentions set alike.
+template <typename Args>
+static void common_params(AttnParams* p, const Args* a, int q_tokens) {
+  p->batch = a->batch;
+  p->q_tokens = q_tokens;
+  p->group = a->q_heads / a->kv_heads;
+  p->gp = pack_of(p->group);
+  p->head_groups = a->q_heads / p->gp;
+  p->tt = 128 / p->gp;
+  p->min_steps = 2;
+  // a zero scale would turn masked scores (-inf) into NaN; the smallest one gives the same weights
+  p->c = std::max(std::fabs(a->scale) * 1.4426950408889634f, 1e-30f);
+  p->neg = a->scale < 0;
+  p->cu_q = a->cu_q;
+  p->q = a->q;
+  p->q_token = a->q_token;
+  p->q_head = a->q_head;
+  p->out = a->out;
+  p->out_token = a->out_token;
+  p->out_head = a->out_head;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p->err = reinterpret_cast<int*>(ws);
+  p->counters = reinterpret_cast<int*>(ws + kAttnCtlBytes);
+  p->partials = reinterpret_cast<float*>(ws + kAttnCtlBytes + kAttnCounterBytes);
+  p->timeout_ns = wait_limit_ns();
+}
+
+static int attn_grid(int* grid) {
+  SVD_CHECK(device_sms(grid));
+  *grid = std::min(*grid, kAttnMaxGrid);
+  return SVDMLP_OK;
+}
+
 static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   if (!a || !a->q || !a->k || !a->v || !a->cu_q || !a->cu_k || !a->out) return SVDMLP_ERR_INVALID_VALUE;
   if (a->batch <= 0 || a->q_tokens <= 0 || a->k_tokens <= 0) return SVDMLP_ERR_INVALID_VALUE;
@@ -146,18 +245,29 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
     return SVDMLP_ERR_ALIGNMENT;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return SVDMLP_ERR_INVALID_VALUE;
   if (a->workspace_bytes < svdmlp_prompt_workspace_bytes()) return SVDMLP_ERR_WORKSPACE;
-  const long long warps = static_cast<long long>(a->q_tokens) * a->q_heads;
-  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
-  if (a->dtype == SVDMLP_BF16) {
-    if (a->head_dim == 128) prompt_rows_kernel<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(*a);
-    else prompt_rows_kernel<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(*a);
-  } else {
-    if (a->head_dim == 128) prompt_rows_kernel<__half, 128><<<grid, 256, 0, s>>>(*a);
-    else prompt_rows_kernel<__half, 64><<<grid, 256, 0, s>>>(*a);
-  }
-  SVD_CUDA(cudaGetLastError());
-  count_launch();
-  return SVDMLP_OK;
+  AttnParams p{};
+  common_params(&p, a, a->q_tokens);
+  p.k_tokens = a->k_tokens;
+  p.causal = a->causal != 0;
+  // one row tile holds the mean request: alternate key steps instead of leaving the second tile empty
+  p.alt = static_cast<int64_t>(a->q_tokens) * p.gp <= 128ll * a->batch;
+  p.cu_k = a->cu_k;
+  p.k = a->k;
+  p.v = a->v;
+  p.k_token = a->k_token;
+  p.k_head = a->k_head;
+  p.v_token = a->v_token;
+  p.v_head = a->v_head;
+  int grid = 0;
+  SVD_CHECK(attn_grid(&grid));
+  CUtensorMap mq, mk, mv;
+  SVD_CHECK(query_map(&mq, a->dtype, a->q, a->q_tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
+  const int64_t dims[3] = {a->head_dim, a->kv_heads, a->k_tokens};
+  const int64_t ks[3] = {1, a->k_head, a->k_token}, vs[3] = {1, a->v_head, a->v_token};
+  const int box[3] = {64, 1, kAttnStep};
+  SVD_CHECK(attn_map(&mk, a->dtype, a->k, 3, dims, ks, box));
+  SVD_CHECK(attn_map(&mv, a->dtype, a->v, 3, dims, vs, box));
+  return dispatch_attention<false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
 }
 
 static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
@@ -175,18 +285,33 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
     return SVDMLP_ERR_ALIGNMENT;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return SVDMLP_ERR_INVALID_VALUE;
   if (a->workspace_bytes < svdmlp_tree_workspace_bytes(a->head_dim)) return SVDMLP_ERR_WORKSPACE;
-  const long long warps = static_cast<long long>(a->tokens) * a->q_heads;
-  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
-  if (a->dtype == SVDMLP_BF16) {
-    if (a->head_dim == 128) tree_rows_kernel<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(*a);
-    else tree_rows_kernel<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(*a);
-  } else {
-    if (a->head_dim == 128) tree_rows_kernel<__half, 128><<<grid, 256, 0, s>>>(*a);
-    else tree_rows_kernel<__half, 64><<<grid, 256, 0, s>>>(*a);
-  }
-  SVD_CUDA(cudaGetLastError());
-  count_launch();
-  return SVDMLP_OK;
+  AttnParams p{};
+  common_params(&p, a, a->tokens);
+  p.tree = 1;
+  p.alt = static_cast<int64_t>(a->max_tree) * p.gp <= 128;
+  p.lens = a->lens;
+  p.table = a->table;
+  p.mask = reinterpret_cast<const long long*>(a->mask);
+  p.ld_table = a->ld_table;
+  p.block_size = a->block_size;
+  for (p.block_shift = 0; (1 << p.block_shift) < a->block_size;) ++p.block_shift;
+  p.num_blocks = a->num_blocks;
+  p.width = a->table_width;
+  p.k = a->k_cache;
+  p.v = a->v_cache;
+  p.k_token = a->k_block;
+  p.v_token = a->v_block;
+  int grid = 0;
+  SVD_CHECK(attn_grid(&grid));
+  CUtensorMap mq, mk, mv;
+  SVD_CHECK(query_map(&mq, a->dtype, a->q, a->tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
+  const int64_t dims[4] = {a->head_dim, a->block_size, a->kv_heads, a->num_blocks};
+  const int64_t head = static_cast<int64_t>(a->block_size) * a->head_dim;
+  const int64_t ks[4] = {1, a->head_dim, head, a->k_block}, vs[4] = {1, a->head_dim, head, a->v_block};
+  const int box[4] = {64, std::min(a->block_size, kAttnStep), 1, 1};
+  SVD_CHECK(attn_map(&mk, a->dtype, a->k_cache, 4, dims, ks, box));
+  SVD_CHECK(attn_map(&mv, a->dtype, a->v_cache, 4, dims, vs, box));
+  return dispatch_attention<true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
 }
 
 }  // namespace svdmlp
@@ -201,7 +326,7 @@ int svdmlp_page_step(const svdmlp_pages_args* args, void* stream) {
   return svdmlp::pages_impl(args, static_cast<cudaStream_t>(stream));
 }
 
-int64_t svdmlp_prompt_workspace_bytes(void) { return 256; }
+int64_t svdmlp_prompt_workspace_bytes(void) { return svdmlp::attn_workspace<128>(); }
 
 int svdmlp_prompt_attention(const svdmlp_prompt_args* args, void* stream) {
   return svdmlp::prompt_impl(args, static_cast<cudaStream_t>(stream));
@@ -209,7 +334,7 @@ int svdmlp_prompt_attention(const svdmlp_prompt_args* args, void* stream) {
 
 int64_t svdmlp_tree_workspace_bytes(int32_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return SVDMLP_ERR_SHAPE_MISMATCH;
-  return 256;
+  return head_dim == 128 ? svdmlp::attn_workspace<128>() : svdmlp::attn_workspace<64>();
 }
 
 int svdmlp_tree_attention(const svdmlp_tree_args* args, void* stream) {
