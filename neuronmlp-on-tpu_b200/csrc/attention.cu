@@ -173,35 +173,38 @@ static constexpr int64_t kAttnCtlBytes = 256, kAttnCounterBytes = 1 << 20;  // a
 template <int D>
 static int64_t attn_workspace() {
   return kAttnCtlBytes + kAttnCounterBytes +
-         static_cast<int64_t>(std::min(planning_sms(), kAttnMaxGrid)) * 2 * AttnCfg<D>::PART_FLOATS * 4;
+         static_cast<int64_t>(std::min(planning_sms(), kAttnMaxGrid)) * 2 * AttnCfg<D, true>::PART_FLOATS * 4;
 }
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool PAIR>
 static int launch_attention(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnParams& p,
                             int grid, cudaStream_t s) {
+  constexpr int SMEM = AttnCfg<D, PAIR>::SMEM_BYTES;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
   int dev = 0;
   SVD_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    SVD_CUDA(cudaFuncSetAttribute(attention_kernel<T, D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  AttnCfg<D>::SMEM_BYTES));
+    SVD_CUDA(cudaFuncSetAttribute(attention_kernel<T, D, PAGED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  attention_kernel<T, D, PAGED><<<static_cast<unsigned>(grid), kAttnThreads, AttnCfg<D>::SMEM_BYTES, s>>>(q, k, v, p);
+  attention_kernel<T, D, PAGED, PAIR><<<static_cast<unsigned>(grid), kAttnThreads, SMEM, s>>>(q, k, v, p);
   SVD_CUDA(cudaGetLastError());
   count_launch();
   return SVDMLP_OK;
 }
 
-template <bool PAGED>
+template <bool PAGED, bool PAIR>
 static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                               const AttnParams& p, int grid, cudaStream_t s) {
   if (dtype == SVDMLP_BF16)
-    return head_dim == 128 ? launch_attention<__nv_bfloat16, 128, PAGED>(q, k, v, p, grid, s)
-                           : launch_attention<__nv_bfloat16, 64, PAGED>(q, k, v, p, grid, s);
-  return head_dim == 128 ? launch_attention<__half, 128, PAGED>(q, k, v, p, grid, s)
-                         : launch_attention<__half, 64, PAGED>(q, k, v, p, grid, s);
+    return head_dim == 128 ? launch_attention<__nv_bfloat16, 128, PAGED, PAIR>(q, k, v, p, grid, s)
+                           : launch_attention<__nv_bfloat16, 64, PAGED, PAIR>(q, k, v, p, grid, s);
+  return head_dim == 128 ? launch_attention<__half, 128, PAGED, PAIR>(q, k, v, p, grid, s)
+                         : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, s);
 }
+
+// Keys of one ring slot, the height of the k and v boxes.
+static int slot_keys(bool pair) { return pair ? AttnCfg<128, true>::KEYS : AttnCfg<128, false>::KEYS; }
 
 // What both attentions set alike.
 template <typename Args>
@@ -212,7 +215,7 @@ static void common_params(AttnParams* p, const Args* a, int q_tokens) {
   p->gp = pack_of(p->group);
   p->head_groups = a->q_heads / p->gp;
   p->tt = 128 / p->gp;
-  p->min_steps = 2;
+  p->snap = 4;
   // a zero scale would turn masked scores (-inf) into NaN; the smallest one gives the same weights
   p->c = std::max(std::fabs(a->scale) * 1.4426950408889634f, 1e-30f);
   p->neg = a->scale < 0;
@@ -249,8 +252,8 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   common_params(&p, a, a->q_tokens);
   p.k_tokens = a->k_tokens;
   p.causal = a->causal != 0;
-  // one row tile holds the mean request: alternate key steps instead of leaving the second tile empty
-  p.alt = static_cast<int64_t>(a->q_tokens) * p.gp <= 128ll * a->batch;
+  // one row tile holds the mean request: two workers instead of a second row tile that would mostly be empty
+  const bool pair = static_cast<int64_t>(a->q_tokens) * p.gp > 128ll * a->batch;
   p.cu_k = a->cu_k;
   p.k = a->k;
   p.v = a->v;
@@ -264,10 +267,11 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->q_tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[3] = {a->head_dim, a->kv_heads, a->k_tokens};
   const int64_t ks[3] = {1, a->k_head, a->k_token}, vs[3] = {1, a->v_head, a->v_token};
-  const int box[3] = {64, 1, kAttnStep};
+  const int box[3] = {64, 1, slot_keys(pair)};
   SVD_CHECK(attn_map(&mk, a->dtype, a->k, 3, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v, 3, dims, vs, box));
-  return dispatch_attention<false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
+  return pair ? dispatch_attention<false, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
+              : dispatch_attention<false, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
 }
 
 static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
@@ -288,7 +292,7 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   AttnParams p{};
   common_params(&p, a, a->tokens);
   p.tree = 1;
-  p.alt = static_cast<int64_t>(a->max_tree) * p.gp <= 128;
+  const bool pair = static_cast<int64_t>(a->max_tree) * p.gp > 128;
   p.lens = a->lens;
   p.table = a->table;
   p.mask = reinterpret_cast<const long long*>(a->mask);
@@ -308,10 +312,11 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   const int64_t dims[4] = {a->head_dim, a->block_size, a->kv_heads, a->num_blocks};
   const int64_t head = static_cast<int64_t>(a->block_size) * a->head_dim;
   const int64_t ks[4] = {1, a->head_dim, head, a->k_block}, vs[4] = {1, a->head_dim, head, a->v_block};
-  const int box[4] = {64, std::min(a->block_size, kAttnStep), 1, 1};
+  const int box[4] = {64, std::min(a->block_size, slot_keys(pair)), 1, 1};
   SVD_CHECK(attn_map(&mk, a->dtype, a->k_cache, 4, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v_cache, 4, dims, vs, box));
-  return dispatch_attention<true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
+  return pair ? dispatch_attention<true, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
+              : dispatch_attention<true, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
 }
 
 }  // namespace svdmlp

@@ -6,23 +6,27 @@
 // the group for tt = 128 / gp tokens, row = token * gp + head (a group of more
 // than 64 heads is taken head by head).  Packing the group lets one tile of k
 // and v serve every head that shares it, fills the 128 rows of the MMA when
-// there are few tokens, and narrows the causal diagonal to tt tokens.
+// there are few tokens, and narrows the causal diagonal to tt tokens.  Keys are
+// walked in steps of 128.
 //
-// A unit is one (request, head group, token tile) of two row tiles ("pair"), or
-// of one row tile whose key steps alternate between the two softmax groups
-// ("alt", for requests of at most 128 rows, where a second row tile would be
-// empty).  Its keys are walked in steps of 128.
+// Two schedules (PAIR, chosen by the host).  A unit is one (request, head
+// group, token tile).  PAIR: a unit has two row tiles, which share every k and
+// v tile; for requests of more than 128 rows.  Otherwise a unit has one row
+// tile, and the CTA holds two independent workers, each with its own ring, MMA
+// warp and TMA warp, so that one's loads and epilogues lie beside the other's
+// products: a second row tile would be empty, and the bytes of k and v bound.
 //
 // Work.  All steps of all units form one line, cut into equal pieces, one per
-// CTA (persistent, one per SM): every CTA computes the cut itself from the
-// request lengths on the device, so ragged lengths, long prompts and a single
-// long context load every SM alike.  A unit that a cut divides leaves fp32
-// partials (maximum, sum, unnormalised output) in the workspace; the CTA that
-// arrives last at the unit's counter joins them in the order of the keys, so
-// results do not depend on the order of arrival.
+// worker (persistent, one CTA per SM): every CTA computes its cuts itself from
+// the request lengths on the device, so ragged lengths, long prompts and a
+// single long context load every SM alike.  A cut inside a short unit moves to
+// the unit's start.  A unit that a cut divides leaves fp32 partials (maximum,
+// sum, unnormalised output) in the workspace; the worker that arrives last at
+// the unit's counter joins them in the order of the keys, so results do not
+// depend on the order of arrival.
 //
-// Roles (384 threads): two softmax warpgroups, one thread per row; an MMA warp;
-// a TMA warp.  TMEM (512 columns): scores S0, S1 (128 each; the probabilities
+// Roles (384 threads): two softmax warpgroups, one thread per row; MMA and TMA
+// warps.  TMEM (512 columns): scores S0, S1 (128 each; the probabilities
 // overwrite them as 16-bit pairs and are the A operand of the second product)
 // and outputs O0, O1.  The MMA warp issues P0 V(j), Q0 K(j+1), P1 V(j),
 // Q1 K(j+1): while one group turns scores into probabilities, the tensor pipe
@@ -49,8 +53,8 @@ constexpr float kAttnLazy = 8.0f;     // growth of the maximum (log2) that a sta
 struct AttnParams {
   int batch, q_tokens, k_tokens;
   int head_groups, gp, group;         // units per token tile; query heads per unit; query heads per kv head
-  int tt, alt, causal, tree;
-  int min_steps;                      // fewest steps a CTA takes
+  int tt, causal, tree;
+  int snap;                           // units of up to this many steps are not divided
   float c;                            // |scale| log2(e)
   int neg;                            // scale < 0
   const int *cu_q, *cu_k;             // packed keys
@@ -67,17 +71,21 @@ struct AttnParams {
   unsigned long long timeout_ns;
 };
 
-template <int D>
+template <int D, bool PAIR>
 struct AttnCfg {
   static constexpr int HALVES = D / 64;
-  static constexpr int TILE_BYTES = kAttnStep * D * 2;      // one k or v tile, or one row tile of q
-  static constexpr int SLOTS = D == 128 ? 5 : 8;
-  static constexpr int OFF_KV = 2 * TILE_BYTES;
-  static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE_BYTES;
-  static constexpr int OFF_XCHG = TILE_BYTES;               // alt: the second row tile's place is free
+  static constexpr int WORKERS = PAIR ? 1 : 2;              // per CTA
+  static constexpr int Q_BYTES = 128 * D * 2;               // one row tile of q
+  static constexpr int KEYS = PAIR ? 128 : 64;              // keys of one ring slot
+  static constexpr int SUBS = kAttnStep / KEYS;             // slots of k (and of v) per step
+  static constexpr int SLOT_BYTES = KEYS * D * 2;
+  static constexpr int HALF_BYTES = KEYS * 128;             // 64 elements of the head for every key of a slot
+  static constexpr int SLOTS = (D == 128 ? 5 : 10) * (PAIR ? 1 : 2) / WORKERS;  // per worker
+  static constexpr int OFF_KV = 2 * Q_BYTES;
+  static constexpr int OFF_BAR = OFF_KV + WORKERS * SLOTS * SLOT_BYTES;
   static constexpr int SMEM_BYTES = OFF_BAR + 3072;         // the ring begins on 1024 bytes (checked in the kernel)
-  static constexpr int PART_ROWS = 256;
-  static constexpr int PART_FLOATS = PART_ROWS * (D + 2);   // one partial slot: output, maxima, sums
+  static constexpr int PART_ROWS = PAIR ? 256 : 128;
+  static constexpr int PART_FLOATS = PART_ROWS * (D + 2);   // one partial: output, maxima, sums
 };
 
 enum AttnSite : int {
@@ -89,12 +97,11 @@ enum AttnSite : int {
 // K-major B tiles use make_sw128_desc.  v is the B operand of the second
 // product with its rows (keys) along K: MN-major, 64 head elements (128 bytes)
 // per row, eight-row groups 1024 bytes apart along K (stride byte offset), the
-// next 64 elements of the head a whole [128 x 64] tile away (leading byte
-// offset).
-SVD_DEV uint64_t make_sw128_mn_desc(uint32_t saddr) {
+// next 64 elements of the head `lead` bytes away (leading byte offset).
+SVD_DEV uint64_t make_sw128_mn_desc(uint32_t saddr, uint32_t lead) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>((kAttnStep * 128) >> 4) << 16;
+  d |= static_cast<uint64_t>(lead >> 4) << 16;
   d |= static_cast<uint64_t>(1024u >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
@@ -214,22 +221,20 @@ SVD_DEV AttnSeq load_seq(const AttnParams& p, int b) {
   return s;
 }
 
-SVD_DEV int unit_tokens(const AttnParams& p) { return p.alt ? p.tt : 2 * p.tt; }
 // keys that the first t tokens of the request can see
 SVD_DEV int keys_of(const AttnParams& p, const AttnSeq& s, int t) { return p.causal ? min(s.m, max(s.first + t, 0)) : s.m; }
 SVD_DEV int steps_of(int keys) { return (keys + kAttnStep - 1) / kAttnStep; }
-SVD_DEV int tiles_of(const AttnParams& p, const AttnSeq& s) { return (s.n + unit_tokens(p) - 1) / unit_tokens(p); }
-// Steps of token tile i: at least one, so that rows which see no key are written too.
-SVD_DEV int tile_steps(const AttnParams& p, const AttnSeq& s, int i) {
-  return max(1, steps_of(keys_of(p, s, min((i + 1) * unit_tokens(p), s.n))));
+SVD_DEV int tiles_of(const AttnSeq& s, int w) { return (s.n + w - 1) / w; }
+// Steps of token tile i of w tokens: at least one, so that rows which see no key are written too.
+SVD_DEV int tile_steps(const AttnParams& p, const AttnSeq& s, int w, int i) {
+  return max(1, steps_of(keys_of(p, s, min((i + 1) * w, s.n))));
 }
 // Steps of the tiles before tile i (i <= tiles).
-SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int i) {
+SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int w, int i) {
   if (!p.causal) return static_cast<long long>(i) * max(1, steps_of(s.m));
-  const int w = unit_tokens(p), tiles = tiles_of(p, s);
   long long sum = 0;
-  if (i == tiles && i > 0) {  // the last tile may be cut short
-    sum = tile_steps(p, s, i - 1);
+  if (i > 0 && i * w >= s.n) {  // the last tile may be cut short
+    sum = tile_steps(p, s, w, i - 1);
     --i;
   }
   // tiles whose keys fit one step, then ceil((first + (k + 1) w) / step)
@@ -242,15 +247,34 @@ SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int i) {
   return sum;
 }
 
-// The segment of a unit that this CTA works on, and where the CTA goes next.
+// A place on the line of steps: global step, and the unit it lies in.
+struct AttnCut {
+  long long at;
+  int b, h, tile, j;
+};
+
+// The segment of a unit that a worker is at, and where it goes next.
+template <bool PAIR>
 struct AttnWalk {
   AttnSeq s;
   int b, h, tile, tiles, j0, j1, steps;
-  long long at, end;   // global step of the segment's first step; end of this CTA's piece
+  long long at, end;   // global step of the segment's first step; end of this worker's piece
 
-  SVD_DEV bool open(const AttnParams& p) {
+  SVD_DEV static int tokens(const AttnParams& p) { return PAIR ? 2 * p.tt : p.tt; }
+  SVD_DEV bool start(const AttnParams& p, const AttnCut& from, long long to) {
+    at = from.at;
+    end = to;
     if (at >= end) return false;
-    steps = tile_steps(p, s, tile);
+    b = from.b;
+    h = from.h;
+    tile = from.tile;
+    j0 = from.j;
+    s = load_seq(p, b);
+    tiles = tiles_of(s, tokens(p));
+    return open(p);
+  }
+  SVD_DEV bool open(const AttnParams& p) {
+    steps = tile_steps(p, s, tokens(p), tile);
     const long long left = end - at;
     j1 = left < steps - j0 ? j0 + static_cast<int>(left) : steps;
     return true;
@@ -264,34 +288,22 @@ struct AttnWalk {
       if (++h == p.head_groups) {
         h = 0;
         do {
-          if (++b >= p.batch) {
-            at = end;
-            return false;
-          }
+          if (++b >= p.batch) return false;
           s = load_seq(p, b);
         } while (s.n == 0);
-        tiles = tiles_of(p, s);
+        tiles = tiles_of(s, tokens(p));
       }
     }
     return open(p);
   }
-  // rows of row tile i: first token, tokens, steps
-  SVD_DEV int tile_t0(const AttnParams& p, int i) const { return tile * unit_tokens(p) + (p.alt ? 0 : i * p.tt); }
-  SVD_DEV int tile_tokens(const AttnParams& p, int i) const { return max(0, min(p.tt, s.n - tile_t0(p, i))); }
+  // row tile i: its first token, tokens, steps
+  SVD_DEV int t0(const AttnParams& p, int i) const { return tile * tokens(p) + (PAIR ? i * p.tt : 0); }
+  SVD_DEV int row_tokens(const AttnParams& p, int i) const { return max(0, min(p.tt, s.n - t0(p, i))); }
   SVD_DEV int row_steps(const AttnParams& p, int i) const {
-    const int nt = tile_tokens(p, i);
-    return nt == 0 ? 0 : steps_of(keys_of(p, s, tile_t0(p, i) + nt));
-  }
-  // Whether softmax group i works on step j, and whether anything does.
-  SVD_DEV bool active(const AttnParams& p, int i, int j, int steps_i) const {
-    return j < steps_i && (!p.alt || ((j - j0) & 1) == i);
+    const int nt = row_tokens(p, i);
+    return nt == 0 ? 0 : steps_of(keys_of(p, s, t0(p, i) + nt));
   }
 };
-
-// Places of the segment's tiles in the ring (loads since the segment began).
-// pair: K0 V0 K1 V1 ...; alt: K0 K1 V0 K2 V1 ... (two score tiles in flight).
-SVD_DEV int k_place(int alt, int i) { return !alt ? 2 * i : i == 0 ? 0 : 2 * i - 1; }
-SVD_DEV int v_place(int alt, int i, int n) { return !alt ? 2 * i + 1 : i == n - 1 ? 2 * i + 1 : 2 * i + 2; }
 
 // ------------------------------------------------------- the row-wise path
 // The output of one row over the keys [j_lo, j_hi) of its segment, a warp per
@@ -340,14 +352,14 @@ __device__ __noinline__ void attn_row(const AttnParams& p, const AttnSeq& s, int
 
 // -------------------------------------------------------------- the kernel
 struct AttnShared {
-  uint64_t q_full, q_empty, xchg, drain;
-  uint64_t s_full[2], p_ready[2], pv_done[2];
-  uint64_t kv_full[8], kv_empty[8];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], pv_done[2], xchg[2], drain[2];
+  uint64_t kv_full[20], kv_empty[20];
   uint32_t tmem;
-  int abort_flag, last;
-  int start_b, start_h, start_tile, start_j;
-  long long start, end, total, per;
+  int abort_flag, last[2];
+  AttnCut cut[3];
+  long long per;
   long long scan[kAttnThreads / 32];
+  long long rem[3];
   float m[256], l[256];         // joining: per-row maximum and 1 / sum
 };
 
@@ -357,92 +369,117 @@ SVD_DEV bool warp_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, int s
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, site, honour_abort));
 }
 
-// Every CTA finds its piece of the line of steps.
-SVD_DEV void find_piece(const AttnParams& p, AttnShared* sh) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int NW = kAttnThreads / 32;
-  long long base = 0, total = 0;
-  // first the total, then (second round) the request that holds the piece's first step
-  for (int round = 0; round < 2; ++round) {
-    base = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kAttnThreads) {
+SVD_DEV long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// Every CTA finds its own cuts of the line of steps, one per warpgroup: the
+// first steps of its workers and the end of the last one's piece.
+template <int WORKERS, bool PAIR>
+SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
+  const int k = threadIdx.x >> 7, tid = threadIdx.x & 127;
+  const int lane = tid & 31, warp = tid >> 5;
+  if (k > WORKERS) return;
+  const int w = AttnWalk<PAIR>::tokens(p);
+  long long* scan = sh->scan + k * 4;
+  const int rounds = p.batch <= 128 ? 1 : 2;  // more requests than threads: first the total, then the place
+  long long total = 0, at = -1;
+  for (int round = 0; round < rounds; ++round) {
+    long long base = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 128) {
       const int b = b0 + tid;
-      long long mine = 0, unit = 0;
-      AttnSeq s{};
+      long long mine = 0;
+      unsigned unit = 0;
       if (b < p.batch) {
-        s = load_seq(p, b);
-        unit = s.n > 0 ? steps_before(p, s, tiles_of(p, s)) : 0;
-        mine = unit * p.head_groups;
+        const AttnSeq s = load_seq(p, b);
+        if (s.n > 0) {
+          const long long steps = steps_before(p, s, w, tiles_of(s, w));
+          unit = static_cast<unsigned>(steps);
+          mine = steps * p.head_groups;
+        }
       }
       long long inc = mine;
+#pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += up;
       }
-      if (lane == 31) sh->scan[warp] = inc;
-      __syncthreads();
+      if (lane == 31) scan[warp] = inc;
+      named_barrier_sync(1 + k, 128);
       long long before = base, all = 0;
-      for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += sh->scan[w];
-        all += sh->scan[w];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (x < warp) before += scan[x];
+        all += scan[x];
       }
       before += inc - mine;
-      __syncthreads();
       base += all;
-      if (p.batch <= kAttnThreads) total = base;  // one chunk: the total is known at once
-      if (round == 1 || p.batch <= kAttnThreads) {
-        const long long per = max(static_cast<long long>(p.min_steps), (total + gridDim.x - 1) / gridDim.x);
-        const long long start = per * blockIdx.x;
-        if (tid == 0) {
-          sh->per = per;
-          sh->start = start;
-          sh->end = min(start + per, total);
-        }
-        if (start >= before && start < before + mine) {
-          const long long in = start - before;
-          sh->start_b = b;
-          sh->start_h = static_cast<int>(in / unit);
-          const long long rem = in - (in / unit) * unit;
-          int lo = 0, hi = tiles_of(p, s);  // the last tile with at most rem steps before it
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (steps_before(p, s, mid) <= rem) lo = mid;
-            else hi = mid;
+      if (b0 + 128 < p.batch || round + 1 < rounds) named_barrier_sync(1 + k, 128);
+      if (round + 1 == rounds) {
+        if (rounds == 1) total = base;
+        if (at < 0) {
+          const long long workers = static_cast<long long>(gridDim.x) * WORKERS;
+          const long long per = max(1ll, quotient(total + workers - 1, workers));
+          at = min(per * (static_cast<long long>(blockIdx.x) * WORKERS + k), total);
+          if (tid == 0) {
+            if (k == 0) sh->per = per;
+            sh->cut[k].at = at;
           }
-          sh->start_tile = lo;
-          sh->start_j = static_cast<int>(rem - steps_before(p, s, lo));
+        }
+        if (at >= before && at < before + mine) {
+          const long long in = at - before;
+          const long long h = quotient(in, unit);
+          sh->cut[k].b = b;
+          sh->cut[k].h = static_cast<int>(h);
+          sh->rem[k] = in - h * unit;
         }
       }
     }
     total = base;
-    if (p.batch <= kAttnThreads) break;
+  }
+  named_barrier_sync(1 + k, 128);
+  if (warp == 0 && at < total) {
+    // the last tile with at most `rem` steps before it, 32 candidates at a time
+    const long long rem = sh->rem[k];
+    const int b = sh->cut[k].b;
+    const AttnSeq s = load_seq(p, b);
+    int lo = 0, hi = tiles_of(s, w);  // lo is at or before it, hi beyond
+    if (!p.causal) {
+      lo = static_cast<int>(quotient(rem, max(1, steps_of(s.m))));
+    } else {
+      while (hi - lo > 1) {
+        const int stride = (hi - lo + 31) / 32;
+        const int x = lo + lane * stride;
+        const bool below = x < hi && steps_before(p, s, w, x) <= rem;
+        const int n = __popc(__ballot_sync(0xffffffffu, below));  // lane 0 always
+        hi = min(hi, lo + n * stride);
+        lo += (n - 1) * stride;
+      }
+    }
+    if (lane == 0) {
+      int j = static_cast<int>(rem - steps_before(p, s, w, lo));
+      if (j > 0 && tile_steps(p, s, w, lo) <= p.snap) {
+        sh->cut[k].at = at - j;
+        j = 0;
+      }
+      sh->cut[k].tile = lo;
+      sh->cut[k].j = j;
+    }
   }
 }
 
-SVD_DEV AttnWalk first_walk(const AttnParams& p, const AttnShared* sh) {
-  AttnWalk w{};
-  w.at = sh->start;
-  w.end = sh->end;
-  if (w.at < w.end) {
-    w.b = sh->start_b;
-    w.h = sh->start_h;
-    w.tile = sh->start_tile;
-    w.j0 = sh->start_j;
-    w.s = load_seq(p, w.b);
-    w.tiles = tiles_of(p, w.s);
-  }
-  return w;
-}
-
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool PAIR>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p) {
-  using Cfg = AttnCfg<D>;
+  using Cfg = AttnCfg<D, PAIR>;
+  using Walk = AttnWalk<PAIR>;
   constexpr bool F16 = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t smem[];
   AttnShared* sh = reinterpret_cast<AttnShared*>(smem + Cfg::OFF_BAR);
   static_assert(Cfg::OFF_BAR + sizeof(AttnShared) <= Cfg::SMEM_BYTES && Cfg::SMEM_BYTES <= 232448, "shared memory");
+  static_assert(Cfg::WORKERS * Cfg::SLOTS <= 20, "barriers");
   if ((smem_addr(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
     if (threadIdx.x == 0) atomicCAS(p.err, 0, SITE_ATTN_ALIGN);
     return;
@@ -451,16 +488,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int lane = static_cast<int>(lane_id());
 
   if (threadIdx.x == 0) {
-    mbar_init(&sh->q_full, 1);
-    mbar_init(&sh->q_empty, 1);
-    mbar_init(&sh->xchg, 256);
-    mbar_init(&sh->drain, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh->q_full[i], 1);
+      mbar_init(&sh->q_empty[i], 1);
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_ready[i], 128);
       mbar_init(&sh->pv_done[i], 1);
+      mbar_init(&sh->xchg[i], PAIR ? 256 : 128);
+      mbar_init(&sh->drain[i], 1);
     }
-    for (int i = 0; i < Cfg::SLOTS; ++i) {
+    for (int i = 0; i < Cfg::WORKERS * Cfg::SLOTS; ++i) {
       mbar_init(&sh->kv_full[i], 1);
       mbar_init(&sh->kv_empty[i], 1);
     }
@@ -475,237 +512,264 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     tmem_relinquish();
     tc_fence_before();
   }
-  find_piece(p, sh);
+  find_cuts<Cfg::WORKERS, PAIR>(p, sh);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
   const WaitCtx ctx{&sh->abort_flag, p.err, p.timeout_ns};
-  AttnWalk w = first_walk(p, sh);
-
-  // rows of no request give zeros
-  {
-    const int lo = min(max(p.cu_q[0], 0), p.q_tokens), hi = min(max(p.cu_q[p.batch], lo), p.q_tokens);
-    const int heads = p.head_groups * p.gp;
-    const long long rows = static_cast<long long>(lo + p.q_tokens - hi) * heads;
-    for (long long r = blockIdx.x * static_cast<long long>(kAttnThreads) + threadIdx.x; r < rows;
-         r += static_cast<long long>(gridDim.x) * kAttnThreads) {
-      const int t = static_cast<int>(r / heads), h = static_cast<int>(r % heads);
-      T* dst = static_cast<T*>(p.out) + static_cast<long long>(t < lo ? t : t - lo + hi) * p.out_token + h * p.out_head;
-      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
-    }
-  }
+  // softmax group, MMA warp (8, 10) and TMA warp (9, 11) of worker wk
+  const int wk = PAIR ? 0 : warp >= 8 ? (warp - 8) >> 1 : warp >> 2;
+  Walk w;
+  bool more = w.start(p, sh->cut[wk], sh->cut[wk + 1].at);
 
   if (warp >= 8) {
     reg_dealloc<88>();
-    if (warp == 9) {
+    uint8_t* ring = smem + Cfg::OFF_KV + wk * Cfg::SLOTS * Cfg::SLOT_BYTES;
+    uint64_t* kv_full = sh->kv_full + wk * Cfg::SLOTS;
+    uint64_t* kv_empty = sh->kv_empty + wk * Cfg::SLOTS;
+    if ((warp & 1) != 0 && (!PAIR || warp == 9)) {
       // ------------------------------------------------------------ TMA warp
-      int ld = 0, seg = 0;
+      int slot = 0, seg = 0;
+      uint32_t phase = 1;  // parity of the next kv_empty wait: the first round finds every slot free
+      int ld = 0;
       bool ok = true;
-      const int q_rows = p.tt * p.gp;
-      const uint32_t tile_bytes = Cfg::TILE_BYTES;
-      for (bool more = w.open(p); more && ok; more = w.next(p), ++seg) {
-        if (!warp_wait(&sh->q_empty, (seg & 1) ^ 1, ctx, SITE_ATTN_Q_EMPTY)) break;
+      for (; more && ok; more = w.next(p), ++seg) {
+        if (!warp_wait(&sh->q_empty[wk], (seg & 1) ^ 1, ctx, SITE_ATTN_Q_EMPTY)) break;
         if (lane == 0) {
-          const int qt = p.alt ? 1 : 2;
-          mbar_arrive_expect_tx(&sh->q_full, static_cast<uint32_t>(qt * Cfg::HALVES * q_rows * 128));
-          for (int i = 0; i < qt; ++i)
+          constexpr int QT = PAIR ? 2 : 1;
+          mbar_arrive_expect_tx(&sh->q_full[wk], static_cast<uint32_t>(QT * Cfg::HALVES * p.tt * p.gp * 128));
+          for (int i = 0; i < QT; ++i)
             for (int hf = 0; hf < Cfg::HALVES; ++hf)
-              tma_load_4d_at(&map_q, &sh->q_full, smem + i * Cfg::TILE_BYTES + hf * (kAttnStep * 128), hf * 64, 0, w.h,
-                             w.s.q0 + w.tile_t0(p, i));
+              tma_load_4d_at(&map_q, &sh->q_full[wk], smem + (wk + i) * Cfg::Q_BYTES + hf * (128 * 128), hf * 64, 0, w.h,
+                             w.s.q0 + w.t0(p, i));
         }
         const int kv_head = w.h * p.gp / p.group;
-        const int n = w.j1 - w.j0;
-        // one tile of k or v into the next slot of the ring
-        const auto load = [&](const CUtensorMap* map, int j) -> bool {
-          const int slot = ld % Cfg::SLOTS;
-          if (!warp_wait(&sh->kv_empty[slot], static_cast<uint32_t>(ld / Cfg::SLOTS & 1) ^ 1u, ctx, SITE_ATTN_KV_EMPTY))
-            return false;
-          ++ld;
-          uint8_t* dst = smem + Cfg::OFF_KV + slot * Cfg::TILE_BYTES;
-          if (lane == 0) mbar_arrive_expect_tx(&sh->kv_full[slot], tile_bytes);
-          __syncwarp();
-          if constexpr (PAGED) {
-            // a lane per block; a block the table does not name is read out of range, as zeros
-            const int rows = min(p.block_size, kAttnStep);
-            if (lane * rows < kAttnStep) {
-              const int key = j * kAttnStep + lane * rows;
-              const int entry = key >> p.block_shift;
-              int page = -1;
-              if (key < w.s.m) page = p.table[w.b * p.ld_table + entry];
-              if (page < 0 || page >= p.num_blocks) page = p.num_blocks;
-              for (int hf = 0; hf < Cfg::HALVES; ++hf)
-                tma_load_4d_at(map, &sh->kv_full[slot], dst + hf * (kAttnStep * 128) + lane * rows * 128, hf * 64,
-                               key & (p.block_size - 1), kv_head, page);
+        for (int j = w.j0; j < w.j1 && ok; ++j) {
+#pragma unroll 1
+          for (int x = 0; x < 2 * Cfg::SUBS && ok; ++x) {  // k, then v
+            const CUtensorMap* map = x < Cfg::SUBS ? &map_k : &map_v;
+            const int sub = x < Cfg::SUBS ? x : x - Cfg::SUBS;
+            const int key0 = j * kAttnStep + sub * Cfg::KEYS;
+            if (sub > 0 && key0 >= w.s.m) continue;        // nothing there
+            if (!(ok = warp_wait(&kv_empty[slot], phase, ctx, SITE_ATTN_KV_EMPTY))) break;
+            uint8_t* dst = ring + slot * Cfg::SLOT_BYTES;
+            if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], Cfg::SLOT_BYTES);
+            __syncwarp();
+            if constexpr (PAGED) {
+              // a lane per block; a block the table does not name is read out of range, as zeros
+              const int rows = min(p.block_size, Cfg::KEYS);
+              if (lane * rows < Cfg::KEYS) {
+                const int key = key0 + lane * rows;
+                int page = -1;
+                if (key < w.s.m) page = p.table[w.b * p.ld_table + (key >> p.block_shift)];
+                if (page < 0 || page >= p.num_blocks) page = p.num_blocks;
+                for (int hf = 0; hf < Cfg::HALVES; ++hf)
+                  tma_load_4d_at(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES + lane * rows * 128, hf * 64,
+                                 key & (p.block_size - 1), kv_head, page);
+              }
+            } else {
+              if (lane == 0)
+                for (int hf = 0; hf < Cfg::HALVES; ++hf)
+                  tma_load_3d(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES, hf * 64, kv_head, w.s.k0 + key0);
             }
-          } else {
-            if (lane == 0)
-              for (int hf = 0; hf < Cfg::HALVES; ++hf)
-                tma_load_3d(map, &sh->kv_full[slot], dst + hf * (kAttnStep * 128), hf * 64, kv_head,
-                            w.s.k0 + j * kAttnStep);
-          }
-          return true;
-        };
-        if (!p.alt) {
-          for (int i = 0; i < n && ok; ++i) ok = load(&map_k, w.j0 + i) && load(&map_v, w.j0 + i);
-        } else {
-          ok = load(&map_k, w.j0);
-          for (int i = 0; i < n && ok; ++i) {
-            if (i + 1 < n) ok = load(&map_k, w.j0 + i + 1);
-            ok = ok && load(&map_v, w.j0 + i);
+            ++ld;
+            if (++slot == Cfg::SLOTS) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
       }
       // every load in flight has landed before the CTA ends
       for (int sl = 0; sl < Cfg::SLOTS; ++sl)
         if (ld > sl) {
-          const int last = sl + (ld - 1 - sl) / Cfg::SLOTS * Cfg::SLOTS;
-          mbar_wait(&sh->kv_full[sl], static_cast<uint32_t>(last / Cfg::SLOTS & 1), ctx, SITE_ATTN_DRAIN, false);
+          const int round = (ld - 1 - sl) / Cfg::SLOTS;
+          mbar_wait(&kv_full[sl], static_cast<uint32_t>(round & 1), ctx, SITE_ATTN_DRAIN, false);
         }
-      if (seg > 0) mbar_wait(&sh->q_full, static_cast<uint32_t>((seg - 1) & 1), ctx, SITE_ATTN_DRAIN, false);
-    } else if (warp == 8) {
+      if (seg > 0) mbar_wait(&sh->q_full[wk], static_cast<uint32_t>((seg - 1) & 1), ctx, SITE_ATTN_DRAIN, false);
+    } else if ((warp & 1) == 0 && (!PAIR || warp == 8)) {
       // ------------------------------------------------------------ MMA warp
-      constexpr uint32_t idesc_s = make_idesc_16bit(128, kAttnStep, F16);
+      constexpr int G0 = 0, GN = PAIR ? 2 : 1;  // row tiles this warp serves
+      constexpr uint32_t idesc_s = make_idesc_16bit(128, Cfg::KEYS, F16);
       constexpr uint32_t idesc_o = make_idesc_16bit(128, D, F16) | kIdescBMnMajor;
-      int ld = 0, seg = 0;
-      int n_p[2] = {0, 0};  // probability tiles consumed, per group
+      int slot = 0, seg = 0;
+      uint32_t phase = 0;
+      int n_p[GN] = {};  // probability tiles consumed, per row tile
       bool ok = true;
-      const auto slot_of = [&](int place) { return (ld + place) % Cfg::SLOTS; };
-      const auto wait_full = [&](int place) {
-        const int x = ld + place;
-        return warp_wait(&sh->kv_full[x % Cfg::SLOTS], static_cast<uint32_t>(x / Cfg::SLOTS & 1), ctx, SITE_ATTN_KV_FULL);
+      // the next slot of the ring, in the order of the loads
+      const auto take = [&]() -> int {
+        if (!(ok = warp_wait(&kv_full[slot], phase, ctx, SITE_ATTN_KV_FULL))) return slot;
+        const int got = slot;
+        if (++slot == Cfg::SLOTS) {
+          slot = 0;
+          phase ^= 1;
+        }
+        return got;
       };
-      const auto release = [&](int place) {
-        if (lane == 0) umma_commit(&sh->kv_empty[slot_of(place)]);
+      const auto release = [&](int sl) {
+        if (lane == 0) umma_commit(&kv_empty[sl]);
       };
-      const auto scores = [&](int i, int place) {  // S_i = Q_i K^T
+      const auto scores = [&](int i, int sl, int sub) {  // S_i = Q_i K^T, the columns of one slot
         if (lane == 0) {
-          const uint32_t a = smem_addr(smem + (p.alt ? 0 : i) * Cfg::TILE_BYTES);
-          const uint32_t bk = smem_addr(smem + Cfg::OFF_KV + slot_of(place) * Cfg::TILE_BYTES);
+          const uint32_t a = smem_addr(smem + (wk + i) * Cfg::Q_BYTES);
+          const uint32_t bk = smem_addr(ring + sl * Cfg::SLOT_BYTES);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * (kAttnStep * 128) + (k % 4) * 32;
-            umma_f16kind(tmem + i * 128, make_sw128_desc(a + off), make_sw128_desc(bk + off), idesc_s, k > 0);
-          }
-          umma_commit(&sh->s_full[i]);
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16kind(tmem + (wk + i) * 128 + sub * Cfg::KEYS,
+                         make_sw128_desc(a + (k / 4) * (128 * 128) + (k % 4) * 32),
+                         make_sw128_desc(bk + (k / 4) * Cfg::HALF_BYTES + (k % 4) * 32), idesc_s, k > 0);
         }
       };
-      const auto values = [&](int i, int place, bool first) {  // O_i (+)= P_i V
+      const auto values = [&](int i, int sl, int sub, bool first) {  // O_i (+)= P_i V
         if (lane == 0) {
-          const uint32_t bv = smem_addr(smem + Cfg::OFF_KV + slot_of(place) * Cfg::TILE_BYTES);
+          const uint32_t bv = smem_addr(ring + sl * Cfg::SLOT_BYTES);
 #pragma unroll
-          for (int k = 0; k < kAttnStep / 16; ++k)
-            umma_f16kind_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, make_sw128_mn_desc(bv + k * 2048), idesc_o,
-                            !first || k > 0);
-          umma_commit(&sh->pv_done[i]);
+          for (int k = 0; k < Cfg::KEYS / 16; ++k)
+            umma_f16kind_ts(tmem + 256 + (wk + i) * D, tmem + (wk + i) * 128 + (sub * (Cfg::KEYS / 16) + k) * 8,
+                            make_sw128_mn_desc(bv + k * 2048, Cfg::HALF_BYTES), idesc_o, !first || k > 0);
         }
       };
       // v rows behind the last key are other requests' or nobody's: zeros
-      const auto clean = [&](int place, int j) {
-        const int valid = w.s.m - j * kAttnStep;
-        if (valid < kAttnStep) {
-          uint8_t* t = smem + Cfg::OFF_KV + slot_of(place) * Cfg::TILE_BYTES;
-          for (int x = max(valid, 0) * 8 + lane; x < kAttnStep * 8; x += 32)
+      const auto clean = [&](int sl, int key0) {
+        const int valid = w.s.m - key0;
+        if (valid < Cfg::KEYS) {
+          uint8_t* t = ring + sl * Cfg::SLOT_BYTES;
+          for (int x = max(valid, 0) * 8 + lane; x < Cfg::KEYS * 8; x += 32)
             for (int hf = 0; hf < Cfg::HALVES; ++hf)
-              *reinterpret_cast<uint4*>(t + hf * (kAttnStep * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(t + hf * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
           __syncwarp();
         }
       };
-      for (bool more = w.open(p); more && ok; more = w.next(p), ++seg) {
-        const int n = w.j1 - w.j0;
-        const int st[2] = {w.row_steps(p, 0), w.row_steps(p, 1)};
-        const int last_place = 2 * n;
-        bool started[2] = {false, false};
-        ok = warp_wait(&sh->q_full, seg & 1, ctx, SITE_ATTN_Q);
-        if (!ok) break;
-        tc_fence_after();
-        // the first score tiles
-        for (int x = 0; x < (p.alt ? min(n, 2) : 1) && ok; ++x) {
-          const int pl = k_place(p.alt, x);
-          ok = wait_full(pl);
-          if (!ok) break;
-          tc_fence_after();
-          for (int i = 0; i < 2; ++i)
-            if (w.active(p, i, w.j0 + x, st[i])) scores(i, pl);
-          release(pl);
-        }
-        const int ahead = p.alt ? 2 : 1;
-        for (int x = 0; x < n && ok; ++x) {
-          const int j = w.j0 + x;
-          const int pv = v_place(p.alt, x, n), pk = k_place(p.alt, x + ahead);
-          const bool more_k = x + ahead < n;
+      // slots of step j that were loaded
+      const auto subs_of = [&](int j) {
+        int n = 1;
+        while (n < Cfg::SUBS && j * kAttnStep + n * Cfg::KEYS < w.s.m) ++n;
+        return n;
+      };
+      for (; more && ok; more = w.next(p), ++seg) {
+        int st[GN];
+        bool started[GN] = {};
+#pragma unroll
+        for (int i = 0; i < GN; ++i) st[i] = w.row_steps(p, i);
+        if (!(ok = warp_wait(&sh->q_full[wk], seg & 1, ctx, SITE_ATTN_Q))) break;
+        for (int j = w.j0; j <= w.j1 && ok; ++j) {
+          // v of step j - 1 and k of step j, row tile by row tile
+          const bool do_v = j > w.j0, do_k = j < w.j1;
+          int sv[Cfg::SUBS], sk[Cfg::SUBS];
+          const int nv = do_v ? subs_of(j - 1) : 0, nk = do_k ? subs_of(j) : 0;
           bool have_v = false, have_k = false;
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (w.active(p, i, j, st[i])) {
-              ok = warp_wait(&sh->p_ready[i], n_p[i] & 1, ctx, SITE_ATTN_P);
-              if (!ok) break;
+#pragma unroll
+          for (int i = G0; i < GN; ++i) {
+            if (ok && do_v && j - 1 < st[i]) {
+              ok = warp_wait(&sh->p_ready[wk + i], n_p[i] & 1, ctx, SITE_ATTN_P);
               ++n_p[i];
               if (!have_v) {
-                ok = wait_full(pv);
-                if (!ok) break;
-                clean(pv, j);
+#pragma unroll
+                for (int x = 0; x < Cfg::SUBS; ++x)
+                  if (ok && x < nv) {
+                    sv[x] = take();
+                    if (ok) clean(sv[x], (j - 1) * kAttnStep + x * Cfg::KEYS);
+                  }
                 have_v = true;
               }
-              tc_fence_after();
-              values(i, pv, !started[i]);
-              started[i] = true;
+              if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < Cfg::SUBS; ++x)
+                  if (x < nv) values(i, sv[x], x, !started[i] && x == 0);
+                started[i] = true;
+                if (lane == 0) umma_commit(&sh->pv_done[wk + i]);
+                if (!PAIR) {
+#pragma unroll
+                  for (int x = 0; x < Cfg::SUBS; ++x)
+                    if (x < nv) release(sv[x]);
+                }
+              }
             }
-            if (more_k && w.active(p, i, j + ahead, st[i])) {
+            if (ok && do_k && j < st[i]) {
+              if (!have_v && do_v) {  // the ring is taken in order
+#pragma unroll
+                for (int x = 0; x < Cfg::SUBS; ++x)
+                  if (ok && x < nv) sv[x] = take();
+                have_v = true;
+              }
               if (!have_k) {
-                ok = wait_full(pk);
-                if (!ok) break;
+#pragma unroll
+                for (int x = 0; x < Cfg::SUBS; ++x)
+                  if (ok && x < nk) sk[x] = take();
                 have_k = true;
               }
-              tc_fence_after();
-              scores(i, pk);
+              if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < Cfg::SUBS; ++x)
+                  if (x < nk) {
+                    scores(i, sk[x], x);
+                    if (!PAIR) release(sk[x]);
+                  }
+                if (lane == 0) umma_commit(&sh->s_full[wk + i]);
+              }
             }
           }
+          // tiles that nothing used have landed before their slots are handed back
+          if (ok && do_v && !have_v) {
+#pragma unroll
+            for (int x = 0; x < Cfg::SUBS; ++x)
+              if (ok && x < nv) sv[x] = take();
+          }
+          if (ok && do_k && !have_k) {
+#pragma unroll
+            for (int x = 0; x < Cfg::SUBS; ++x)
+              if (ok && x < nk) sk[x] = take();
+          }
           if (!ok) break;
-          // a tile that nothing used has landed before its slot is handed back
-          if (!have_v) ok = wait_full(pv);
-          if (ok && more_k && !have_k) ok = wait_full(pk);
-          if (!ok) break;
-          release(pv);
-          if (more_k) release(pk);
+          const bool spare_v = PAIR || !have_v, spare_k = PAIR || !have_k;
+#pragma unroll
+          for (int x = 0; x < Cfg::SUBS; ++x) {
+            if (spare_v && x < nv) release(sv[x]);
+            if (spare_k && x < nk) release(sk[x]);
+          }
+          if (j == w.j1 - 1 && lane == 0) umma_commit(&sh->q_empty[wk]);  // the last product with q is issued
         }
-        if (!ok) break;
-        if (lane == 0) umma_commit(&sh->q_empty);
-        ld += last_place;
       }
-      if (lane == 0) umma_commit(&sh->drain);
+      if (lane == 0) umma_commit(&sh->drain[wk]);
       __syncwarp();
-      mbar_wait(&sh->drain, 0, ctx, SITE_ATTN_DRAIN, false);
+      mbar_wait(&sh->drain[wk], 0, ctx, SITE_ATTN_DRAIN, false);
     }
   } else {
     // -------------------------------------------------------- softmax groups
     reg_alloc<208>();
-    const int i = warp >> 2;                          // group
+    const int i = warp >> 2;                          // group: row tile, S and O
     const int r = threadIdx.x & 127;                  // row of the tile, lane of TMEM
+    const int ti = PAIR ? i : 0;                      // row tile of the unit
+    const int gtid = PAIR ? threadIdx.x : r;          // thread of the worker
+    constexpr int GT = PAIR ? 256 : 128;              // threads of a worker
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + i * 128, t_o = tmem + lanes + 256 + i * D;
     const int row_token = r / p.gp, row_head = r - row_token * p.gp;
     int n_s = 0, n_x = 0;                             // score tiles taken; exchanges
     bool ok = true;
-    const auto meet = [&]() {                         // all 256 softmax threads
-      mbar_arrive(&sh->xchg);
-      const bool k = warp_wait(&sh->xchg, n_x & 1, ctx, SITE_ATTN_XCHG);
+    const auto meet = [&]() {                         // all threads of the worker
+      mbar_arrive(&sh->xchg[wk]);
+      const bool k = warp_wait(&sh->xchg[wk], n_x & 1, ctx, SITE_ATTN_XCHG);
       ++n_x;
       return k;
     };
-    for (bool more = w.open(p); more; more = w.next(p)) {
-      const int steps_i = w.row_steps(p, i);
-      const int t0 = w.tile_t0(p, i), token = t0 + row_token;
-      const bool row_ok = row_token < w.tile_tokens(p, i);
+    for (; more; more = w.next(p)) {
+      const int steps_i = w.row_steps(p, ti);
+      const int t0 = w.t0(p, ti), token = t0 + row_token;
+      const bool row_ok = row_token < w.row_tokens(p, ti);
+      const bool warp_ok = __any_sync(0xffffffffu, row_ok);
       // keys below `open` are seen by every row of the tile, keys from `sees` on by none of this row (outside a mask)
-      const int open = p.tree ? w.s.first : p.causal ? w.s.first + t0 + 1 : w.s.m;
-      const int sees = p.tree ? (p.mask != nullptr ? min(w.s.first, w.s.m) : min(w.s.first + token + 1, w.s.m))
-                              : p.causal ? min(w.s.first + token + 1, w.s.m) : w.s.m;
+      const int open = min(w.s.m, p.tree ? w.s.first : p.causal ? w.s.first + t0 + 1 : w.s.m);
+      const int sees = min(w.s.m, p.tree ? (p.mask != nullptr ? w.s.first : w.s.first + token + 1)
+                                         : p.causal ? w.s.first + token + 1 : w.s.m);
       const unsigned long long bits = p.mask != nullptr && row_ok ? p.mask[w.s.q0 + token] : 0;
       float m = -INFINITY, l = 0.f;                   // m in units of the scores
       bool some = false;
-      const int stride = p.alt ? 2 : 1;
-      const int first_j = w.j0 + (p.alt ? i : 0), last_j = min(w.j1, steps_i);
-      for (int j = first_j; j < last_j; j += stride) {
+      const int last_j = min(w.j1, steps_i);
+      for (int j = w.j0; j < last_j; ++j) {
         unsigned bad_pages = 0;
         if constexpr (PAGED) {
           const int rows = min(p.block_size, kAttnStep);
@@ -718,6 +782,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           bad_pages = __ballot_sync(0xffffffffu, bad);
         }
         if (!(ok = warp_wait(&sh->s_full[i], n_s & 1, ctx, SITE_ATTN_S))) break;
+        if (!warp_ok) {                               // rows of nobody: their probabilities stay what they are
+          mbar_arrive(&sh->p_ready[i]);
+          ++n_s;
+          continue;
+        }
         tc_fence_after();
         float s[128];
 #pragma unroll
@@ -728,7 +797,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int x = 0; x < 128; ++x) s[x] = -s[x];
         }
         const int rel = j * kAttnStep;
-        if (rel + kAttnStep > min(open, w.s.m) || bad_pages != 0) {
+        if (rel + kAttnStep > open || bad_pages != 0) {
           // one bit per key of the step
           uint32_t vis[4];
 #pragma unroll
@@ -741,25 +810,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const int at = w.s.first - rel;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int sh_by = at - 32 * x;          // bit 0 of the tree in this word's coordinates
+              const int by = at - 32 * x;             // bit 0 of the tree in this word's coordinates
               uint32_t part = 0;
-              if (sh_by > -64 && sh_by < 32)
-                part = sh_by >= 0 ? static_cast<uint32_t>(bits << sh_by) : static_cast<uint32_t>(bits >> -sh_by);
+              if (by > -64 && by < 32) part = by >= 0 ? static_cast<uint32_t>(bits << by) : static_cast<uint32_t>(bits >> -by);
               const int end = w.s.m - rel - 32 * x;   // keys that exist
               part &= end >= 32 ? 0xffffffffu : end > 0 ? (1u << end) - 1u : 0u;
               vis[x] |= part;
             }
           }
           if constexpr (PAGED) {
-            if (bad_pages != 0) {
-              const int rows = min(p.block_size, kAttnStep);
-              for (unsigned rest = bad_pages; rest != 0; rest &= rest - 1) {
-                const int lo = (__ffs(rest) - 1) * rows;
+            const int rows = min(p.block_size, kAttnStep);
+            for (unsigned rest = bad_pages; rest != 0; rest &= rest - 1) {
+              const int lo = (__ffs(rest) - 1) * rows;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const int a = max(lo - 32 * x, 0), z = min(lo + rows - 32 * x, 32);
-                  if (a < z) vis[x] &= ~((z - a == 32 ? 0xffffffffu : (1u << (z - a)) - 1u) << a);
-                }
+              for (int x = 0; x < 4; ++x) {
+                const int a = max(lo - 32 * x, 0), z = min(lo + rows - 32 * x, 32);
+                if (a < z) vis[x] &= ~((z - a == 32 ? 0xffffffffu : (1u << (z - a)) - 1u) << a);
               }
             }
           }
@@ -827,96 +893,64 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       // ---------------------------------------------------- the segment's end
       const bool whole = w.j0 == 0 && w.j1 == w.steps;
-      float m_out = m == -INFINITY ? -INFINITY : m * p.c, l_out = l;
-      float w0 = 1.f, w1 = 0.f;                       // alt: weights of the groups' outputs
-      bool has0 = some, has1 = false;
-      if (p.alt) {
-        float* x = reinterpret_cast<float*>(smem + Cfg::OFF_XCHG);
-        x[i * 128 + r] = m_out;
-        x[256 + i * 128 + r] = l;
-        if (!(ok = meet())) break;
-        tc_fence_after();
-        const float m0 = x[r], m1 = x[128 + r];
-        const float l0 = x[256 + r], l1 = x[384 + r];
-        has0 = true;                                  // the first step is group 0's
-        has1 = w.j1 - w.j0 > 1;
-        if (steps_i <= w.j0) has0 = has1 = false;     // no key at all
-        m_out = fmaxf(m0, m1);
-        const float safe = m_out == -INFINITY ? 0.f : m_out;
-        w0 = exp2_approx(m0 - safe);
-        w1 = exp2_approx(m1 - safe);
-        l_out = l0 * w0 + l1 * w1;
-      }
-      const int c_lo = p.alt ? i * (D / 2) : 0, c_hi = p.alt ? c_lo + D / 2 : D;
-      const float inv = l_out == 0.f ? 0.f : 1.f / l_out;
-      const int row = (p.alt ? 0 : i * 128) + r;
+      const float base = m == -INFINITY ? 0.f : m * p.c;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int row = ti * 128 + r;
       const int head = w.h * p.gp + row_head, kv_head = w.h * p.gp / p.group;
-      float* part = nullptr;
-      long long unit0 = w.at - w.j0;
-      if (!whole)
-        part = p.partials + (static_cast<long long>(blockIdx.x) * 2 + (w.at == sh->start ? 0 : 1)) * Cfg::PART_FLOATS;
+      // partials of this worker: one for the unit that it begins, one for the unit that it goes on with
+      float* part = p.partials + ((static_cast<long long>(blockIdx.x) * Cfg::WORKERS + wk) * 2 + (w.j0 == 0 ? 1 : 0)) *
+                                     Cfg::PART_FLOATS;
       T* dst = static_cast<T*>(p.out) + static_cast<long long>(w.s.q0 + token) * p.out_token + head * p.out_head;
-      float probe = 0.f;                              // NaN when any output is not finite
+      if (warp_ok) {
+        float probe = 0.f;                            // NaN when any output is not finite
 #pragma unroll 1
-      for (int x = c_lo; x < c_hi; x += 32) {
-        float v[32];
-        if (p.alt) {
-          uint32_t o0[32], o1[32];
-          tmem_ld_x32(tmem + lanes + 256 + x, o0);
-          tmem_ld_x32(tmem + lanes + 256 + D + x, o1);
-          tmem_ld_wait();
-#pragma unroll
-          for (int y = 0; y < 32; ++y)
-            v[y] = (has0 ? w0 * __uint_as_float(o0[y]) : 0.f) + (has1 ? w1 * __uint_as_float(o1[y]) : 0.f);
-        } else {
+        for (int x = 0; x < D; x += 32) {
+          float v[32];
           tmem_ld_x32(t_o + x, reinterpret_cast<uint32_t(&)[32]>(v));
           tmem_ld_wait();
-          if (!has0) {
+          if (!some) {
 #pragma unroll
             for (int y = 0; y < 32; ++y) v[y] = 0.f;
           }
-        }
 #pragma unroll
-        for (int y = 0; y < 32; ++y) probe = fmaf(v[y], 0.f, probe);
-        if (row_ok) {
-          if (whole) {
+          for (int y = 0; y < 32; ++y) probe = fmaf(v[y], 0.f, probe);
+          if (row_ok) {
+            if (whole) {
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              uint4 o;
-              o.x = pack_pair<T>(v[y] * inv, v[y + 1] * inv);
-              o.y = pack_pair<T>(v[y + 2] * inv, v[y + 3] * inv);
-              o.z = pack_pair<T>(v[y + 4] * inv, v[y + 5] * inv);
-              o.w = pack_pair<T>(v[y + 6] * inv, v[y + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + x + y) = o;
+              for (int y = 0; y < 32; y += 8) {
+                uint4 o;
+                o.x = pack_pair<T>(v[y] * inv, v[y + 1] * inv);
+                o.y = pack_pair<T>(v[y + 2] * inv, v[y + 3] * inv);
+                o.z = pack_pair<T>(v[y + 4] * inv, v[y + 5] * inv);
+                o.w = pack_pair<T>(v[y + 6] * inv, v[y + 7] * inv);
+                *reinterpret_cast<uint4*>(dst + x + y) = o;
+              }
+            } else {
+#pragma unroll
+              for (int y = 0; y < 32; y += 4)
+                __stcg(reinterpret_cast<float4*>(part) + ((x + y) >> 2) * Cfg::PART_ROWS + row,
+                       make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]));
             }
-          } else {
-#pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              __stcg(reinterpret_cast<float4*>(part) + ((x + y) >> 2) * Cfg::PART_ROWS + row,
-                     make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]));
           }
         }
-      }
-      if (!whole && row_ok && c_lo == 0) {
-        __stcg(part + Cfg::PART_ROWS * D + row, m_out);
-        __stcg(part + Cfg::PART_ROWS * (D + 1) + row, l_out);
-      }
-      // rows that a masked place may have reached: over again, key by key
-      unsigned redo = __ballot_sync(0xffffffffu, row_ok && probe != 0.f);
-      while (redo != 0) {
-        const int src = __ffs(redo) - 1;
-        redo &= redo - 1;
-        const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
-        const int rw = __shfl_sync(0xffffffffu, row, src);
-        const float bs = __shfl_sync(0xffffffffu, m_out == -INFINITY ? 0.f : m_out, src);
-        const float iv = __shfl_sync(0xffffffffu, inv, src);
-        float o[D / 32];
-        attn_row<T, D>(p, w.s, w.b, tk, hd, kv_head, w.j0 * kAttnStep, min(w.j1 * kAttnStep, w.s.m), bs, o);
-        __syncwarp();
+        if (!whole && row_ok) {
+          __stcg(part + Cfg::PART_ROWS * D + row, m == -INFINITY ? -INFINITY : base);
+          __stcg(part + Cfg::PART_ROWS * (D + 1) + row, l);
+        }
+        // rows that a masked place may have reached: over again, key by key
+        unsigned redo = __ballot_sync(0xffffffffu, row_ok && probe != 0.f);
+        while (redo != 0) {
+          const int src = __ffs(redo) - 1;
+          redo &= redo - 1;
+          const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
+          const int rw = __shfl_sync(0xffffffffu, row, src);
+          const float bs = __shfl_sync(0xffffffffu, base, src), iv = __shfl_sync(0xffffffffu, inv, src);
+          float o[D / 32];
+          attn_row<T, D>(p, w.s, w.b, tk, hd, kv_head, w.j0 * kAttnStep, min(w.j1 * kAttnStep, w.s.m), bs, o);
+          __syncwarp();
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const int d = lane * (D / 32) + e;
-          if (d >= c_lo && d < c_hi) {
+          for (int e = 0; e < D / 32; ++e) {
+            const int d = lane * (D / 32) + e;
             if (whole)
               static_cast<T*>(p.out)[static_cast<long long>(w.s.q0 + tk) * p.out_token + hd * p.out_head + d] =
                   elem_from_float<T>(o[e] * iv);
@@ -925,65 +959,79 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
       }
-      if (p.alt) {
-        // both groups have read both outputs before either writes new ones
-        tc_fence_before();
-        if (!(ok = meet())) break;
-      }
+      tc_fence_before();
       if (!whole) {
-        // the last CTA of the unit to arrive joins the partials, in the order of the keys
+        // the last worker of the unit to arrive joins the partials, in the order of the keys
         __threadfence();
         if (!(ok = meet())) break;
-        const int c0 = static_cast<int>(unit0 / sh->per), c1 = static_cast<int>((unit0 + w.steps - 1) / sh->per);
-        if (threadIdx.x == 0) {
+        const long long unit0 = w.at - w.j0;
+        const int c0 = static_cast<int>(quotient(unit0, sh->per));
+        const int c1 = static_cast<int>(quotient(unit0 + w.steps - 1, sh->per));
+        if (gtid == 0) {
           const int arrived = atom_add_acq_rel_gpu(&p.counters[c0], 1);
-          sh->last = arrived == c1 - c0;
-          if (sh->last) p.counters[c0] = 0;
+          sh->last[wk] = arrived == c1 - c0;
+          if (arrived == c1 - c0) p.counters[c0] = 0;
         }
         if (!(ok = meet())) break;
-        if (sh->last) {
+        if (sh->last[wk]) {
           __threadfence();
-          const int tid = threadIdx.x;
-          const long long first_slot = (unit0 == static_cast<long long>(c0) * sh->per) ? 2LL * c0 : 2LL * c0 + 1;
-          const auto slot = [&](int cta) -> const float* {
-            return p.partials + (cta == c0 ? first_slot : 2LL * cta) * Cfg::PART_FLOATS;
+          const auto partial = [&](int c) -> const float* {
+            return p.partials + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS;
           };
-          const int tok0 = w.tile_tokens(p, 0), tok1 = p.alt ? 0 : w.tile_tokens(p, 1);
+          const int rows0 = w.row_tokens(p, 0) * p.gp;
+          const int rows = rows0 + (PAIR ? w.row_tokens(p, 1) * p.gp : 0);
+          float* jm = sh->m + wk * 128;
+          float* jl = sh->l + wk * 128;
           // per row: the common maximum and 1 / sum
-          {
-            const int rr = tid;                       // row of the unit
-            const bool there = (rr & 127) / p.gp < (rr < 128 ? tok0 : tok1);
-            float mm = -INFINITY, ll = 0.f;
-            if (there) {
-              for (int cta = c0; cta <= c1; ++cta) mm = fmaxf(mm, __ldcg(slot(cta) + Cfg::PART_ROWS * D + rr));
-              const float safe = mm == -INFINITY ? 0.f : mm;
-              for (int cta = c0; cta <= c1; ++cta)
-                ll += exp2_approx(__ldcg(slot(cta) + Cfg::PART_ROWS * D + rr) - safe) *
-                      __ldcg(slot(cta) + Cfg::PART_ROWS * (D + 1) + rr);
-              mm = safe;
+          if (rows <= 32) {
+            for (int x = gtid >> 5; x < rows; x += GT / 32) {  // a warp per row, lanes over the partials
+              float mm = -INFINITY, ll = 0.f;
+              for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(partial(c) + Cfg::PART_ROWS * D + x));
+              for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+              if (mm == -INFINITY) mm = 0.f;
+              for (int c = c0 + lane; c <= c1; c += 32)
+                ll += exp2_approx(__ldcg(partial(c) + Cfg::PART_ROWS * D + x) - mm) *
+                      __ldcg(partial(c) + Cfg::PART_ROWS * (D + 1) + x);
+              for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+              if (lane == 0) {
+                jm[x] = mm;
+                jl[x] = ll == 0.f ? 0.f : 1.f / ll;
+              }
             }
-            sh->m[rr] = mm;
-            sh->l[rr] = ll == 0.f ? 0.f : 1.f / ll;
+          } else {
+            const int x = gtid;                       // a thread per row
+            if (x < rows0 || (x >= 128 && x - 128 < rows - rows0)) {
+              float mm = -INFINITY, ll = 0.f;
+#pragma unroll 4
+              for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(partial(c) + Cfg::PART_ROWS * D + x));
+              if (mm == -INFINITY) mm = 0.f;
+#pragma unroll 4
+              for (int c = c0; c <= c1; ++c)
+                ll += exp2_approx(__ldcg(partial(c) + Cfg::PART_ROWS * D + x) - mm) *
+                      __ldcg(partial(c) + Cfg::PART_ROWS * (D + 1) + x);
+              jm[x] = mm;
+              jl[x] = ll == 0.f ? 0.f : 1.f / ll;
+            }
           }
           if (!(ok = meet())) break;
-          const int rows0 = tok0 * p.gp, rows = rows0 + tok1 * p.gp;
           const int items = rows * (D / 4);
           constexpr int U = 4;
-          for (int it0 = tid; it0 < items; it0 += 256 * U) {
+          for (int it0 = gtid; it0 < items; it0 += GT * U) {
             float4 acc[U];
             int rowu[U], du[U];
             float mu[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-              const int it = min(it0 + 256 * u, items - 1);
+              const int it = min(it0 + GT * u, items - 1);
               du[u] = it / rows;
               const int x = it - du[u] * rows;
               rowu[u] = x < rows0 ? x : 128 + x - rows0;
-              mu[u] = sh->m[rowu[u]];
+              mu[u] = jm[rowu[u]];
               acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            for (int cta = c0; cta <= c1; ++cta) {
-              const float* sl = slot(cta);
+#pragma unroll 2
+            for (int c = c0; c <= c1; ++c) {
+              const float* sl = partial(c);
               float wt[U];
               float4 o[U];
 #pragma unroll
@@ -1002,10 +1050,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-              if (it0 + 256 * u < items) {
-                const int rr = rowu[u] & 127, tl = rowu[u] >> 7;
-                const float iv = sh->l[rowu[u]];
-                const int tk = w.tile_t0(p, tl) + rr / p.gp, hd = w.h * p.gp + rr % p.gp;
+              if (it0 + GT * u < items) {
+                const int rr = rowu[u] & 127;
+                const float iv = jl[rowu[u]];
+                const int tk = w.t0(p, rowu[u] >> 7) + rr / p.gp, hd = w.h * p.gp + rr % p.gp;
                 uint2 o;
                 o.x = pack_pair<T>(acc[u].x * iv, acc[u].y * iv);
                 o.y = pack_pair<T>(acc[u].z * iv, acc[u].w * iv);
@@ -1020,6 +1068,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   }
 
+  // rows of no request give zeros
+  {
+    const int lo = min(max(p.cu_q[0], 0), p.q_tokens), hi = min(max(p.cu_q[p.batch], lo), p.q_tokens);
+    const int heads = p.head_groups * p.gp;
+    const long long rows = static_cast<long long>(lo + p.q_tokens - hi) * heads;
+    for (long long x = blockIdx.x * static_cast<long long>(kAttnThreads) + threadIdx.x; x < rows;
+         x += static_cast<long long>(gridDim.x) * kAttnThreads) {
+      const int t = static_cast<int>(x / heads), h = static_cast<int>(x % heads);
+      T* dst = static_cast<T*>(p.out) + static_cast<long long>(t < lo ? t : t - lo + hi) * p.out_token + h * p.out_head;
+      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
