@@ -38,42 +38,58 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 # -------------------------------------------------------------------- checks
-def _dtype(t: torch.Tensor) -> int:
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"supported dtypes are bfloat16 and float16, got {t.dtype}")
-    return code
+# A call first takes its arguments through one expression of plain attribute
+# comparisons (a decoding step's launches take a few microseconds each, so the
+# checks have to as well); only where that fails, _refuse_* name what is wrong.
+_stream = torch._C._cuda_getCurrentRawStream
+_device = torch.cuda.current_device
 
 
-def _heads(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """A [tokens, heads, head_dim] CUDA tensor, of the type, device and head size of `like`."""
+def _refuse_dtype(t) -> None:
     if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
-    if t.dim() != 3 or t.shape[1] <= 0 or t.shape[2] <= 0:
-        raise ValueError(f"{name}: expected [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor (the B200 path has no CPU fallback)")
-    if like is not None:
+        raise TypeError(f"expected a torch.Tensor, got {type(t).__name__}")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"supported dtypes are bfloat16 and float16, got {t.dtype}")
+
+
+def _refuse_heads(**tensors: torch.Tensor) -> None:
+    """Raises what is wrong with [tokens, heads, head_dim] tensors; the first sets the type, device and head size."""
+    like = None
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+        if t.dim() != 3 or t.shape[1] <= 0 or t.shape[2] <= 0:
+            raise ValueError(f"{name}: expected [tokens, heads, head_dim], got {tuple(t.shape)}")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (the B200 path has no CPU fallback)")
+        if like is None:
+            _refuse_dtype(t)
+            like = t
         if t.dtype != like.dtype:
             raise TypeError("all inputs must have the same dtype")
         if t.device != like.device:
             raise ValueError("inputs must be CUDA tensors on one device")
         if t.shape[2] != like.shape[2]:
             raise ValueError(f"{name} has head_dim {t.shape[2]}, expected {like.shape[2]}: dimensions do not match")
-    return t if t.stride(2) == 1 else t.contiguous()
 
 
-def _vector_rows(t: torch.Tensor) -> torch.Tensor:
-    """`t`, or a copy of it when its rows do not lie on 16-byte boundaries."""
-    if t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+def _vector_rows(t: torch.Tensor, strides) -> bool:
+    """Whether the kernels read t's rows in place: unit stride in the head, rows on 16-byte boundaries."""
+    return (strides[2] == 1 and not (strides[0] | strides[1]) & 7 and not t.data_ptr() & 15
+            and (strides[0] > 0 or t.shape[0] == 1) and (strides[1] > 0 or t.shape[1] == 1))
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a copy of it that the kernels read in place."""
+    if _vector_rows(t, t.stride()):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}: dimensions do not match")
     if t.device != device:
         raise ValueError("inputs must be CUDA tensors on one device")
@@ -81,7 +97,7 @@ def _index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device:
 
 
 def _offsets(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
     if t.dim() != 1 or t.shape[0] < 2:
         raise ValueError(f"{name} must be [batch + 1], got {tuple(t.shape)}")
@@ -90,7 +106,7 @@ def _offsets(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv_heads: Optional[int]):
+def _refuse_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv_heads: Optional[int]) -> None:
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
@@ -102,11 +118,26 @@ def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv
             raise ValueError("inputs must be CUDA tensors on one device")
         if t.shape[3] != like.shape[2] or (kv_heads is not None and t.shape[1] != kv_heads):
             raise ValueError(f"{name} {tuple(t.shape)} does not match the heads: dimensions do not match")
-        d, b = t.shape[3], t.shape[2]
-        if t.stride(3) != 1 or t.stride(2) != d or t.stride(1) != b * d:
+        if t.stride()[1:] != (t.shape[2] * t.shape[3], t.shape[3], 1):
             raise ValueError(f"{name} must be contiguous inside a block")
     if k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have matching shapes")
+
+
+def _check_caches(k_cache, v_cache, like: torch.Tensor, kv_heads: Optional[int]):
+    """(num_blocks, kv_heads, block_size, stride between k blocks, between v blocks), or an exception."""
+    try:
+        nb, hk, bs, d = shape = k_cache.shape
+        kb, *inner = k_cache.stride()
+        vb, *inner_v = v_cache.stride()
+        if (inner == inner_v == [bs * d, d, 1] and v_cache.shape == shape and nb * hk * bs > 0
+                and d == like.shape[2] and (kv_heads is None or hk == kv_heads)
+                and k_cache.dtype is v_cache.dtype is like.dtype and k_cache.device == v_cache.device == like.device):
+            return nb, hk, bs, kb, vb
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _refuse_caches(k_cache, v_cache, like, kv_heads)
+    raise ValueError("k_cache and v_cache must have matching layouts")
 
 
 def _scale(scale: Optional[float], head_dim: int) -> float:
@@ -117,26 +148,43 @@ def _scale(scale: Optional[float], head_dim: int) -> float:
     return float(scale)
 
 
-def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if tuple(out.shape) != tuple(q.shape) or out.device != q.device:
+def _output(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+    if out.shape != q.shape or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} on {q.device}: dimensions do not match")
     if out.dtype != q.dtype:
         raise TypeError("out must have the inputs' dtype")
-    if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+    if not _vector_rows(out, out.stride()):
         raise ValueError("out must have 16-byte aligned rows")
     return out
 
 
 def _call(fn, args: bytes, device: torch.device, what: str) -> None:
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != _device():
         with torch.cuda.device(device):
-            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(args, _stream(index))
     else:
-        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+        status = fn(args, _stream(index))
     if status:
         _lib.check(status, what)
+
+
+_workspace_need: dict = {}
+
+
+def _workspace(device: torch.device, head_dim: int):
+    """The attention workspace of the device's current stream: the pool that the other operators use."""
+    need = _workspace_need.get((device.index, head_dim))
+    if need is None:
+        lib = _lib.load()
+        with torch.cuda.device(device):
+            need = max(int(lib.svdmlp_prompt_workspace_bytes()), int(lib.svdmlp_tree_workspace_bytes(head_dim)))
+        _workspace_need[device.index, head_dim] = need
+    with ops._ws_lock:
+        ws = ops._ws_pool.get((device.index, _stream(device.index)))
+    if ws is not None and ws.nbytes >= need:
+        return ws
+    return ops.workspace_for(device, need)
 
 
 # -------------------------------------------------------------------- rotary
@@ -194,41 +242,56 @@ def rope_frequencies(head_dim: int, *, base: float = 10000.0, rotary_dim: Option
 
 
 def _rope(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, scale, return_k):
-    q = _heads("q", q)
-    code = _dtype(q)
-    k = _heads("k", k, q)
-    n, h, d = q.shape
-    hk = k.shape[1]
-    device = q.device
-    if k.shape[0] != n:
+    cached = k_cache is not None or v_cache is not None
+    try:
+        n, h, d = q.shape
+        nk, hk, dk = k.shape
+        device, dtype = q.device, q.dtype
+        code = _DTYPES.get(dtype)
+        good = (code is not None and dk == d and h > 0 and hk > 0 and d > 0 and k.dtype is dtype and k.device == device
+                and q.is_cuda and (not cached or (v.dtype is dtype and v.device == device and v.dim() == 3)))
+    except (AttributeError, TypeError, ValueError):
+        good = False
+    if not good:
+        _refuse_heads(q=q, k=k, **({"v": v} if cached else {}))
+        raise ValueError("unsupported arguments")
+    if nk != n:
         raise ValueError("q and k must have the same tokens: dimensions do not match")
     positions = _index("positions", positions, torch.int32, (n,), device)
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32:
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype is not torch.float32:
         raise TypeError("inv_freq must be a float32 tensor")
     if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d or not inv_freq.is_contiguous():
         raise ValueError(f"inv_freq must be [rotary_dim / 2] with rotary_dim at most {d}, got {tuple(inv_freq.shape)}")
     if inv_freq.device != device:
         raise ValueError("inputs must be CUDA tensors on one device")
-    vs = slots_ptr = kc = vc = kb = vb = bs = nb = 0
-    v_strides = (0, 0)
-    if k_cache is not None:
-        v = _heads("v", v, q)
+    q_token, q_head, unit = q.stride()
+    if unit != 1:
+        q = q.contiguous()
+        q_token, q_head, unit = q.stride()
+    k_token, k_head, unit = k.stride()
+    if unit != 1:
+        k = k.contiguous()
+        k_token, k_head, unit = k.stride()
+    v_ptr = slots_ptr = kc = vc = kb = vb = bs = nb = v_token = v_head = 0
+    if cached:
         if v.shape != k.shape:
             raise ValueError("k and v must have matching shapes")
         slots = _index("slots", slots, torch.int64, (n,), device)
-        _caches(k_cache, v_cache, q, hk)
-        vs, slots_ptr, v_strides = v.data_ptr(), slots.data_ptr(), v.stride()
-        kc, vc, kb, vb = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), v_cache.stride(0)
-        nb, bs = k_cache.shape[0], k_cache.shape[2]
-    q_out = torch.empty((n, h, d), dtype=q.dtype, device=device)
-    k_out = torch.empty((n, hk, d), dtype=q.dtype, device=device) if return_k else None
+        nb, _, bs, kb, vb = _check_caches(k_cache, v_cache, q, hk)
+        v_token, v_head, unit = v.stride()
+        if unit != 1:
+            v = v.contiguous()
+            v_token, v_head, unit = v.stride()
+        v_ptr, slots_ptr, kc, vc = v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    q_out = torch.empty((n, h, d), dtype=dtype, device=device)
+    k_out = torch.empty((n, hk, d), dtype=dtype, device=device) if return_k else None
     if n == 0:
         return q_out, k_out
     args = _lib.ROPE_ARGS(code, n, h, hk, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, bs, nb, scale,
-                          q.data_ptr(), k.data_ptr(), vs, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                          v_strides[0], v_strides[1], positions.data_ptr(), slots_ptr, inv_freq.data_ptr(),
-                          q_out.data_ptr(), k_out.data_ptr() if return_k else 0, kc, vc, kb, vb)
-    _call(_lib.load().svdmlp_rope, args, device, "rope")
+                          q.data_ptr(), k.data_ptr(), v_ptr, q_token, q_head, k_token, k_head, v_token, v_head,
+                          positions.data_ptr(), slots_ptr, inv_freq.data_ptr(), q_out.data_ptr(),
+                          k_out.data_ptr() if return_k else 0, kc, vc, kb, vb)
+    _call((_lib._lib or _lib.load()).svdmlp_rope, args, device, "rope")
     return q_out, k_out
 
 
@@ -306,14 +369,14 @@ def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     slots = torch.empty(num_tokens, dtype=torch.int64, device=device)
     whole = torch.empty(num_tokens + 2 * b + 3, dtype=torch.int32, device=device)
     at = whole.data_ptr()
-    positions, cu, lens, left, missing = whole.split((num_tokens, b + 1, b, 1, 1))
+    positions, cu, lens, left, missing = whole.split_with_sizes((num_tokens, b + 1, b, 1, 1))
     cu_at = at + 4 * num_tokens
     lens_at = cu_at + 4 * (b + 1)
     left_at = lens_at + 4 * b
     args = _lib.PAGES_ARGS(b, num_tokens, block_size, width, free_blocks.shape[0], 0, block_table.data_ptr(),
                            block_table.stride(0), seq_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
                            free_count.data_ptr(), slots.data_ptr(), at, cu_at, lens_at, left_at, left_at + 4)
-    _call(_lib.load().svdmlp_page_step, args, device, "page_step")
+    _call((_lib._lib or _lib.load()).svdmlp_page_step, args, device, "page_step")
     return PageStep(slots, positions, cu, lens, left, missing)
 
 
@@ -336,15 +399,22 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     no sequence, give zeros.  `scale` defaults to 1 / sqrt(D).  bf16 or fp16,
     D 64 or 128; the probabilities are rounded to the inputs' type for the
     product with v, statistics and sums are fp32."""
-    q = _heads("q", q)
-    code = _dtype(q)
-    k, v = _heads("k", k, q), _heads("v", v, q)
-    if k.shape != v.shape:
-        raise ValueError("k and v must have matching shapes")
-    nq, h, d = q.shape
-    nk, hk = k.shape[0], k.shape[1]
-    _group(q, hk)
-    device = q.device
+    try:
+        nq, h, d = q.shape
+        nk, hk, dk = k.shape
+        device, dtype = q.device, q.dtype
+        code = _DTYPES.get(dtype)
+        good = (code is not None and d == dk and (d == 128 or d == 64) and hk > 0 and h > 0 and h % hk == 0
+                and v.shape == k.shape and k.dtype is dtype and v.dtype is dtype and q.is_cuda
+                and k.device == device and v.device == device)
+    except (AttributeError, TypeError, ValueError):
+        good = False
+    if not good:
+        _refuse_heads(q=q, k=k, v=v)
+        if k.shape != v.shape:
+            raise ValueError("k and v must have matching shapes")
+        _group(q, k.shape[1])
+        raise ValueError("unsupported arguments")
     cu_q = _offsets("cu_q", cu_q, device)
     if cu_k is None:
         if nq != nk:
@@ -355,19 +425,21 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if cu_k.shape != cu_q.shape:
             raise ValueError("cu_q and cu_k must have matching shapes")
     scale = _scale(scale, d)
-    out = _output(out, q)
+    out = torch.empty((nq, h, d), dtype=dtype, device=device) if out is None else _output(out, q)
     if nq == 0:
         return out
     if nk == 0:
         return out.zero_()
-    q, k, v = _vector_rows(q), _vector_rows(k), _vector_rows(v)
-    lib = _lib.load()
-    ws = ops.workspace_for(device, lib.svdmlp_prompt_workspace_bytes())
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    ws = _workspace(device, d)
+    q_token, q_head, _ = q.stride()
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    o_token, o_head, _ = out.stride()
     args = _lib.PROMPT_ARGS(code, cu_q.shape[0] - 1, nq, nk, h, hk, d, 1 if causal else 0, scale, 0, q.data_ptr(),
-                            k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                            v.stride(0), v.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), out.stride(0),
-                            out.stride(1), ws.ptr, ws.nbytes)
-    _call(lib.svdmlp_prompt_attention, args, device, "prompt_attention")
+                            k.data_ptr(), v.data_ptr(), q_token, q_head, k_token, k_head, v_token, v_head,
+                            cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), o_token, o_head, ws.ptr, ws.nbytes)
+    _call((_lib._lib or _lib.load()).svdmlp_prompt_attention, args, device, "prompt_attention")
     return out
 
 
@@ -387,39 +459,47 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     decoding and a chain needs no mask.  `max_tree` is the largest n expected
     (it sizes the tiles; larger trees are still computed).  Rows that see
     nothing give zeros.  The block size is a power of two from 8 to 1024."""
-    q = _heads("q", q)
-    code = _dtype(q)
-    _caches(k_cache, v_cache, q, None)
-    n, h, d = q.shape
-    hk, bs = k_cache.shape[1], k_cache.shape[2]
-    _group(q, hk)
+    try:
+        n, h, d = q.shape
+        device, dtype = q.device, q.dtype
+        code = _DTYPES.get(dtype)
+        good = code is not None and h > 0 and d > 0 and q.is_cuda
+    except (AttributeError, TypeError, ValueError):
+        good = False
+    if not good:
+        _refuse_heads(q=q)
+        raise ValueError("unsupported arguments")
+    nb, hk, bs, kb, vb = _check_caches(k_cache, v_cache, q, None)
+    if h % hk or (d != 128 and d != 64):
+        _group(q, hk)
     if bs & (bs - 1) or not 8 <= bs <= 1024:
         raise ValueError(f"the cache's block size must be a power of two from 8 to 1024, got {bs}")
-    device = q.device
     cu_q = _offsets("cu_q", cu_q, device)
     b = cu_q.shape[0] - 1
     seq_lens = _index("seq_lens", seq_lens, torch.int32, (b,), device)
-    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype is not torch.int32:
         raise TypeError("block_table must be an int32 tensor")
     if block_table.dim() != 2 or block_table.shape[0] != b or block_table.shape[1] <= 0 or block_table.stride(1) != 1:
         raise ValueError(f"block_table must be row-major [{b}, width], got {tuple(block_table.shape)}: "
                          "dimensions do not match")
     if block_table.device != device:
         raise ValueError("inputs must be CUDA tensors on one device")
+    mask_ptr = 0
     if tree_mask is not None:
         tree_mask = _index("tree_mask", tree_mask, torch.int64, (n,), device)
+        mask_ptr = tree_mask.data_ptr()
     ops._positive("max_tree", max_tree)
     scale = _scale(scale, d)
-    out = _output(out, q)
+    out = torch.empty((n, h, d), dtype=dtype, device=device) if out is None else _output(out, q)
     if n == 0:
         return out
-    q = _vector_rows(q)
-    lib = _lib.load()
-    ws = ops.workspace_for(device, lib.svdmlp_tree_workspace_bytes(d))
-    args = _lib.TREE_ARGS(code, b, n, h, hk, d, bs, k_cache.shape[0], block_table.shape[1], max_tree, scale, 0,
-                          q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-                          k_cache.stride(0), v_cache.stride(0), block_table.data_ptr(), block_table.stride(0),
-                          seq_lens.data_ptr(), cu_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
-                          out.data_ptr(), out.stride(0), out.stride(1), ws.ptr, ws.nbytes)
-    _call(lib.svdmlp_tree_attention, args, device, "tree_attention")
+    q = _rows(q)
+    ws = _workspace(device, d)
+    q_token, q_head, _ = q.stride()
+    o_token, o_head, _ = out.stride()
+    args = _lib.TREE_ARGS(code, b, n, h, hk, d, bs, nb, block_table.shape[1], max_tree, scale, 0, q.data_ptr(), q_token,
+                          q_head, k_cache.data_ptr(), v_cache.data_ptr(), kb, vb, block_table.data_ptr(),
+                          block_table.stride(0), seq_lens.data_ptr(), cu_q.data_ptr(), mask_ptr, out.data_ptr(), o_token,
+                          o_head, ws.ptr, ws.nbytes)
+    _call((_lib._lib or _lib.load()).svdmlp_tree_attention, args, device, "tree_attention")
     return out
