@@ -203,8 +203,8 @@ static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, con
                          : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, s);
 }
 
-// Keys of one ring slot, the height of the k and v boxes.
-static int slot_keys(bool pair) { return pair ? AttnCfg<128, true>::KEYS : AttnCfg<128, false>::KEYS; }
+// Keys per step.
+static int attn_step(bool pair) { return pair ? AttnCfg<128, true>::STEP : AttnCfg<128, false>::STEP; }
 
 // What both attentions set alike.
 template <typename Args>
@@ -215,10 +215,10 @@ static void common_params(AttnParams* p, const Args* a, int q_tokens) {
   p->gp = pack_of(p->group);
   p->head_groups = a->q_heads / p->gp;
   p->tt = 128 / p->gp;
-  p->snap = 4;
   // a zero scale would turn masked scores (-inf) into NaN; the smallest one gives the same weights
   p->c = std::max(std::fabs(a->scale) * 1.4426950408889634f, 1e-30f);
   p->neg = a->scale < 0;
+  p->wide = (reinterpret_cast<uintptr_t>(a->out) & 31u) == 0 && a->out_token % 16 == 0 && a->out_head % 16 == 0;
   p->cu_q = a->cu_q;
   p->q = a->q;
   p->q_token = a->q_token;
@@ -267,7 +267,8 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->q_tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[3] = {a->head_dim, a->kv_heads, a->k_tokens};
   const int64_t ks[3] = {1, a->k_head, a->k_token}, vs[3] = {1, a->v_head, a->v_token};
-  const int box[3] = {64, 1, slot_keys(pair)};
+  const int step = attn_step(pair), box[3] = {64, 1, step};
+  p.snap = 512 / step;
   SVD_CHECK(attn_map(&mk, a->dtype, a->k, 3, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v, 3, dims, vs, box));
   return pair ? dispatch_attention<false, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
@@ -312,7 +313,8 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   const int64_t dims[4] = {a->head_dim, a->block_size, a->kv_heads, a->num_blocks};
   const int64_t head = static_cast<int64_t>(a->block_size) * a->head_dim;
   const int64_t ks[4] = {1, a->head_dim, head, a->k_block}, vs[4] = {1, a->head_dim, head, a->v_block};
-  const int box[4] = {64, std::min(a->block_size, slot_keys(pair)), 1, 1};
+  const int step = attn_step(pair), box[4] = {64, std::min(a->block_size, step), 1, 1};
+  p.snap = 512 / step;
   SVD_CHECK(attn_map(&mk, a->dtype, a->k_cache, 4, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v_cache, 4, dims, vs, box));
   return pair ? dispatch_attention<true, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)

@@ -7,7 +7,7 @@
 // than 64 heads is taken head by head).  Packing the group lets one tile of k
 // and v serve every head that shares it, fills the 128 rows of the MMA when
 // there are few tokens, and narrows the causal diagonal to tt tokens.  Keys are
-// walked in steps of 128.
+// walked in steps of 64.
 //
 // Two schedules (PAIR, chosen by the host).  A unit is one (request, head
 // group, token tile).  PAIR: a unit has two row tiles, which share every k and
@@ -16,7 +16,8 @@
 // warp and TMA warp, so that one's loads and epilogues lie beside the other's
 // products: a second row tile would be empty, and the bytes of k and v bound.
 //
-// Work.  All steps of all units form one line, cut into equal pieces, one per
+// Work.  The steps of all units, and a few steps' worth for every unit's
+// beginning and end, form one line, cut into equal pieces, one per
 // worker (persistent, one CTA per SM): every CTA computes its cuts itself from
 // the request lengths on the device, so ragged lengths, long prompts and a
 // single long context load every SM alike.  A cut inside a short unit moves to
@@ -26,19 +27,22 @@
 // depend on the order of arrival.
 //
 // Roles (384 threads): two softmax warpgroups, one thread per row; MMA and TMA
-// warps.  TMEM (512 columns): scores S0, S1 (128 each; the probabilities
-// overwrite them as 16-bit pairs and are the A operand of the second product)
-// and outputs O0, O1.  The MMA warp issues P0 V(j), Q0 K(j+1), P1 V(j),
-// Q1 K(j+1): while one group turns scores into probabilities, the tensor pipe
-// works for the other.  The output is rescaled only when a row's maximum grows
-// by more than 8 (in powers of two): a stale base keeps probabilities below
-// 2^8, which the 16-bit types and the fp32 sums hold without loss.
+// warps.  TMEM (512 columns): per group two score tiles of 64 keys (the
+// probabilities overwrite them as 16-bit pairs and are the A operand of the
+// second product) and one output tile.  Scores run two steps ahead: the MMA
+// warp issues P V(j) and then Q K(j + 2), which takes P(j)'s place, while the
+// group already works on the scores of step j + 1, across the ends of units
+// too.  The output is rescaled only when a row's maximum grows by more than 8
+// (in powers of two): a stale base keeps probabilities below 2^8, which the
+// 16-bit types and the fp32 sums hold without loss.
 //
-// What bounds it: at 128 keys x 128 rows a step costs 1024 cycles of the
-// tensor pipe (head_dim 128) and 1024 of the exponential unit; with few rows
-// the bytes of k and v.
+// What bounds it: 64 keys x 128 rows cost 640 cycles of the tensor pipe at
+// head_dim 128 (its shared-memory reads: q and k for 64 columns take 48 cycles
+// per 16 elements where the products take 32) and 512 of the exponential unit;
+// with few rows the bytes of k and v.
 #pragma once
 
+#include <climits>
 #include <type_traits>
 
 #include "rope_pages.cuh"
@@ -46,7 +50,6 @@
 namespace svdmlp {
 
 constexpr int kAttnThreads = 384;
-constexpr int kAttnStep = 128;        // keys per step
 constexpr int kAttnMaxGrid = 512;     // counters and partial slots reserved
 constexpr float kAttnLazy = 8.0f;     // growth of the maximum (log2) that a stale base absorbs
 
@@ -57,6 +60,7 @@ struct AttnParams {
   int snap;                           // units of up to this many steps are not divided
   float c;                            // |scale| log2(e)
   int neg;                            // scale < 0
+  int wide;                           // the output's rows lie on 32-byte boundaries
   const int *cu_q, *cu_k;             // packed keys
   const int *lens, *table;            // paged keys
   const long long* mask;
@@ -76,11 +80,11 @@ struct AttnCfg {
   static constexpr int HALVES = D / 64;
   static constexpr int WORKERS = PAIR ? 1 : 2;              // per CTA
   static constexpr int Q_BYTES = 128 * D * 2;               // one row tile of q
-  static constexpr int KEYS = PAIR ? 128 : 64;              // keys of one ring slot
-  static constexpr int SUBS = kAttnStep / KEYS;             // slots of k (and of v) per step
-  static constexpr int SLOT_BYTES = KEYS * D * 2;
-  static constexpr int HALF_BYTES = KEYS * 128;             // 64 elements of the head for every key of a slot
-  static constexpr int SLOTS = (D == 128 ? 5 : 10) * (PAIR ? 1 : 2) / WORKERS;  // per worker
+  static constexpr int STEP = PAIR ? 128 : 64;              // keys per step
+  static constexpr int SLOT_BYTES = STEP * D * 2;           // k or v of one step
+  static constexpr int HALF_BYTES = STEP * 128;             // 64 elements of the head for every key of a slot
+  static constexpr int SLOTS = D == 128 ? 5 : 8;            // per worker
+  static constexpr int TILES = 128 / STEP;                  // score tiles per group: steps that the scores run ahead
   static constexpr int OFF_KV = 2 * Q_BYTES;
   static constexpr int OFF_BAR = OFF_KV + WORKERS * SLOTS * SLOT_BYTES;
   static constexpr int SMEM_BYTES = OFF_BAR + 3072;         // the ring begins on 1024 bytes (checked in the kernel)
@@ -110,13 +114,44 @@ SVD_DEV uint64_t make_sw128_mn_desc(uint32_t saddr, uint32_t lead) {
 
 constexpr uint32_t kIdescBMnMajor = 1u << 16;
 
-// D[128 x N] (+)= A[128 x 16] B[16 x N], A in TMEM (two 16-bit elements per column).
-SVD_DEV void umma_f16kind_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// The products of one step, issued by one elected lane of a converged warp.
+// Descriptors and addresses are the same in every lane, so that the compiler
+// can keep them in uniform registers: issued from a branch that one lane takes,
+// each MMA cost some 100 cycles of issue, more than it runs for.
+// S[128 x N] = Q[128 x 16 K] K^T, both K-major; the next 64 elements of the head
+// are 16384 (q) and HALF (k) bytes further on.
+template <int K, int HALF>
+SVD_DEV void umma_scores(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc + ((k / 4) * 16384 + (k % 4) * 32) / 16), "l"(b_desc + ((k / 4) * HALF + (k % 4) * 32) / 16),
+        "r"(idesc), "r"(k > 0 ? 1 : 0)
+        : "memory");
+}
+
+// O[128 x N] (+)= P[128 x 64] V[64 x N], P in TMEM (two 16-bit elements per column).
+SVD_DEV void umma_values(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem + k * 8), "l"(b_desc + k * 2048 / 16), "r"(idesc), "r"(k > 0 ? 1u : accumulate)
+        : "memory");
+}
+
+SVD_DEV void umma_commit_elected(uint64_t* bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
       : "memory");
 }
 
@@ -155,10 +190,44 @@ SVD_DEV void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::
 template <int N>
 SVD_DEV void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// 32 bytes as one store (a whole sector), or two where the address is 16-byte aligned only.
+SVD_DEV void store_32(void* at, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
+                      uint32_t h, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(a), "r"(b), "r"(c), "r"(d),
+                 "r"(e), "r"(f), "r"(g), "r"(h)
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(at)[0] = make_uint4(a, b, c, d);
+    reinterpret_cast<uint4*>(at)[1] = make_uint4(e, f, g, h);
+  }
+}
+
 SVD_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations in one instruction.
+SVD_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+SVD_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 template <typename T>
@@ -172,25 +241,30 @@ SVD_DEV uint32_t pack_pair<__half>(float lo, float hi) {
 }
 
 // --------------------------------------------------------------- the cutting
-// sum over i < n of floor((a i + b) / m), a, b >= 0 (the Euclid-like floor sum).
-SVD_DEV long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  long long ans = 0;
-  while (n > 0) {
-    if (a >= m) {
-      ans += (static_cast<long long>(n) * (n - 1) / 2) * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      ans += static_cast<long long>(n) * (b / m);
-      b %= m;
-    }
-    const unsigned long long y = static_cast<unsigned long long>(a) * n + b;
-    if (y < m) break;
-    n = static_cast<unsigned>(y / m);
-    b = static_cast<unsigned>(y % m);
+SVD_DEV long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// sum over i < n of floor((a i + b) / m), a, b >= 0 (the Euclid-like floor sum;
+// M: the first modulus, a power of two).
+template <int M>
+SVD_DEV long long floor_sum(long long n, unsigned a, unsigned b) {
+  long long ans = n * (n - 1) / 2 * (a / M) + n * (b / M);
+  a %= M;
+  b %= M;
+  long long y = a * n + b;
+  unsigned m = M;
+  while (y >= m) {
+    n = quotient(y, m);
+    b = static_cast<unsigned>(y - n * m);
     const unsigned t = m;
     m = a;
     a = t;
+    ans += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    y = a * n + b;
   }
   return ans;
 }
@@ -223,34 +297,44 @@ SVD_DEV AttnSeq load_seq(const AttnParams& p, int b) {
 
 // keys that the first t tokens of the request can see
 SVD_DEV int keys_of(const AttnParams& p, const AttnSeq& s, int t) { return p.causal ? min(s.m, max(s.first + t, 0)) : s.m; }
-SVD_DEV int steps_of(int keys) { return (keys + kAttnStep - 1) / kAttnStep; }
+template <int STEP>
+SVD_DEV int steps_of(int keys) { return (keys + STEP - 1) / STEP; }
 SVD_DEV int tiles_of(const AttnSeq& s, int w) { return (s.n + w - 1) / w; }
 // Steps of token tile i of w tokens: at least one, so that rows which see no key are written too.
+template <int STEP>
 SVD_DEV int tile_steps(const AttnParams& p, const AttnSeq& s, int w, int i) {
-  return max(1, steps_of(keys_of(p, s, min((i + 1) * w, s.n))));
+  return max(1, steps_of<STEP>(keys_of(p, s, min((i + 1) * w, s.n))));
 }
 // Steps of the tiles before tile i (i <= tiles).
+template <int STEP>
 SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int w, int i) {
-  if (!p.causal) return static_cast<long long>(i) * max(1, steps_of(s.m));
+  if (!p.causal) return static_cast<long long>(i) * max(1, steps_of<STEP>(s.m));
   long long sum = 0;
   if (i > 0 && i * w >= s.n) {  // the last tile may be cut short
-    sum = tile_steps(p, s, w, i - 1);
+    sum = tile_steps<STEP>(p, s, w, i - 1);
     --i;
   }
   // tiles whose keys fit one step, then ceil((first + (k + 1) w) / step)
-  const int room = kAttnStep - s.first;
+  const int room = STEP - s.first;
   const int ones = min(i, room >= w ? room / w : 0);
   sum += ones;
   if (i > ones)
-    sum += floor_sum(static_cast<unsigned>(i - ones), kAttnStep, static_cast<unsigned>(w),
-                     static_cast<unsigned>(s.first + (ones + 1) * w + kAttnStep - 1));
+    sum += floor_sum<STEP>(i - ones, static_cast<unsigned>(w),
+                           static_cast<unsigned>(s.first + (ones + 1) * w + STEP - 1));
   return sum;
 }
 
-// A place on the line of steps: global step, and the unit it lies in.
+// On the line a unit is kUnitCost and its steps long: beginning and ending a
+// unit (q, the output) costs about as much as so many steps, and the early
+// tiles of a causal prompt are many units of few steps (measured: without it
+// the CTAs that got those finished 100 us after the others at 8192 tokens).
+constexpr int kUnitCost = 2;
+
+// A place on the line, and the unit and step it lies in.
 struct AttnCut {
   long long at;
   int b, h, tile, j;
+  AttnSeq s;
 };
 
 // The segment of a unit that a worker is at, and where it goes next.
@@ -258,8 +342,9 @@ template <bool PAIR>
 struct AttnWalk {
   AttnSeq s;
   int b, h, tile, tiles, j0, j1, steps;
-  long long at, end;   // global step of the segment's first step; end of this worker's piece
+  long long at, end;   // the segment's place on the line; end of this worker's piece
 
+  static constexpr int STEP = PAIR ? 128 : 64;
   SVD_DEV static int tokens(const AttnParams& p) { return PAIR ? 2 * p.tt : p.tt; }
   SVD_DEV bool start(const AttnParams& p, const AttnCut& from, long long to) {
     at = from.at;
@@ -269,18 +354,18 @@ struct AttnWalk {
     h = from.h;
     tile = from.tile;
     j0 = from.j;
-    s = load_seq(p, b);
+    s = from.s;
     tiles = tiles_of(s, tokens(p));
     return open(p);
   }
   SVD_DEV bool open(const AttnParams& p) {
-    steps = tile_steps(p, s, tokens(p), tile);
-    const long long left = end - at;
+    steps = tile_steps<STEP>(p, s, tokens(p), tile);
+    const long long left = end - at - (j0 == 0 ? kUnitCost : 0);
     j1 = left < steps - j0 ? j0 + static_cast<int>(left) : steps;
     return true;
   }
   SVD_DEV bool next(const AttnParams& p) {
-    at += j1 - j0;
+    at += j1 - j0 + (j0 == 0 ? kUnitCost : 0);
     if (at >= end) return false;
     j0 = 0;
     if (++tile == tiles) {
@@ -301,7 +386,7 @@ struct AttnWalk {
   SVD_DEV int row_tokens(const AttnParams& p, int i) const { return max(0, min(p.tt, s.n - t0(p, i))); }
   SVD_DEV int row_steps(const AttnParams& p, int i) const {
     const int nt = row_tokens(p, i);
-    return nt == 0 ? 0 : steps_of(keys_of(p, s, t0(p, i) + nt));
+    return nt == 0 ? 0 : steps_of<STEP>(keys_of(p, s, t0(p, i) + nt));
   }
 };
 
@@ -352,8 +437,11 @@ __device__ __noinline__ void attn_row(const AttnParams& p, const AttnSeq& s, int
 
 // -------------------------------------------------------------- the kernel
 struct AttnShared {
-  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], pv_done[2], xchg[2], drain[2];
-  uint64_t kv_full[20], kv_empty[20];
+  uint64_t q_full[2], q_empty[2], xchg[2], drain[2];
+  uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];  // per group and score tile
+  uint64_t kv_full[16], kv_empty[16];
+  uint32_t slot_info[16];                // what the TMA warp says of a slot's tile
+  uint32_t score_info[2][2];             // ... and the MMA warp hands on with the scores
   uint32_t tmem;
   int abort_flag, last[2];
   AttnCut cut[3];
@@ -363,15 +451,17 @@ struct AttnShared {
   float m[256], l[256];         // joining: per-row maximum and 1 / sum
 };
 
+// Bits of a slot's info word.
+constexpr uint32_t kInfoRow0 = 1, kInfoRow1 = 2;  // row tiles that the step counts for
+constexpr uint32_t kInfoFirst = 4, kInfoLast = 8; // first, last step of the segment
+constexpr uint32_t kInfoEnd = 16;                 // k: the worker's last step
+constexpr int kInfoValid = 8;                     // v: keys that exist, 0 to 64 (8 bits)
+constexpr int kInfoBad = 16;                      // k: blocks of the step outside the cache (8 bits)
+
 // mbar_wait by a whole warp: every lane gets the same answer, so that no lane
 // is left alone at a warp-wide instruction.
 SVD_DEV bool warp_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, int site, bool honour_abort = true) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, site, honour_abort));
-}
-
-SVD_DEV long long quotient(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
-  return a / b;
 }
 
 // Every CTA finds its own cuts of the line of steps, one per warpgroup: the
@@ -381,6 +471,7 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
   const int k = threadIdx.x >> 7, tid = threadIdx.x & 127;
   const int lane = tid & 31, warp = tid >> 5;
   if (k > WORKERS) return;
+  constexpr int STEP = AttnWalk<PAIR>::STEP;
   const int w = AttnWalk<PAIR>::tokens(p);
   long long* scan = sh->scan + k * 4;
   const int rounds = p.batch <= 128 ? 1 : 2;  // more requests than threads: first the total, then the place
@@ -391,12 +482,14 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
       const int b = b0 + tid;
       long long mine = 0;
       unsigned unit = 0;
+      AttnSeq s{};
       if (b < p.batch) {
-        const AttnSeq s = load_seq(p, b);
+        s = load_seq(p, b);
         if (s.n > 0) {
-          const long long steps = steps_before(p, s, w, tiles_of(s, w));
-          unit = static_cast<unsigned>(steps);
-          mine = steps * p.head_groups;
+          const int tiles = tiles_of(s, w);
+          const long long cost = steps_before<STEP>(p, s, w, tiles) + static_cast<long long>(tiles) * kUnitCost;
+          unit = static_cast<unsigned>(cost);
+          mine = cost * p.head_groups;
         }
       }
       long long inc = mine;
@@ -430,6 +523,7 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
         if (at >= before && at < before + mine) {
           const long long in = at - before;
           const long long h = quotient(in, unit);
+          sh->cut[k].s = s;
           sh->cut[k].b = b;
           sh->cut[k].h = static_cast<int>(h);
           sh->rem[k] = in - h * unit;
@@ -440,27 +534,27 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
   }
   named_barrier_sync(1 + k, 128);
   if (warp == 0 && at < total) {
-    // the last tile with at most `rem` steps before it, 32 candidates at a time
+    // the last tile with at most `rem` before it, 32 candidates at a time
     const long long rem = sh->rem[k];
-    const int b = sh->cut[k].b;
-    const AttnSeq s = load_seq(p, b);
+    const AttnSeq s = sh->cut[k].s;
     int lo = 0, hi = tiles_of(s, w);  // lo is at or before it, hi beyond
     if (!p.causal) {
-      lo = static_cast<int>(quotient(rem, max(1, steps_of(s.m))));
+      lo = static_cast<int>(quotient(rem, max(1, steps_of<STEP>(s.m)) + kUnitCost));
     } else {
       while (hi - lo > 1) {
         const int stride = (hi - lo + 31) / 32;
         const int x = lo + lane * stride;
-        const bool below = x < hi && steps_before(p, s, w, x) <= rem;
+        const bool below = x < hi && steps_before<STEP>(p, s, w, x) + static_cast<long long>(x) * kUnitCost <= rem;
         const int n = __popc(__ballot_sync(0xffffffffu, below));  // lane 0 always
         hi = min(hi, lo + n * stride);
         lo += (n - 1) * stride;
       }
     }
     if (lane == 0) {
-      int j = static_cast<int>(rem - steps_before(p, s, w, lo));
-      if (j > 0 && tile_steps(p, s, w, lo) <= p.snap) {
-        sh->cut[k].at = at - j;
+      const int in = static_cast<int>(rem - steps_before<STEP>(p, s, w, lo) - static_cast<long long>(lo) * kUnitCost);
+      int j = in - kUnitCost;
+      if (j <= 0 || tile_steps<STEP>(p, s, w, lo) <= p.snap) {  // at the unit's start
+        sh->cut[k].at = at - in;
         j = 0;
       }
       sh->cut[k].tile = lo;
@@ -479,7 +573,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   AttnShared* sh = reinterpret_cast<AttnShared*>(smem + Cfg::OFF_BAR);
   static_assert(Cfg::OFF_BAR + sizeof(AttnShared) <= Cfg::SMEM_BYTES && Cfg::SMEM_BYTES <= 232448, "shared memory");
-  static_assert(Cfg::WORKERS * Cfg::SLOTS <= 20, "barriers");
+  static_assert(Cfg::WORKERS * Cfg::SLOTS <= 16, "barriers");
   if ((smem_addr(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
     if (threadIdx.x == 0) atomicCAS(p.err, 0, SITE_ATTN_ALIGN);
     return;
@@ -491,9 +585,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->q_full[i], 1);
       mbar_init(&sh->q_empty[i], 1);
-      mbar_init(&sh->s_full[i], 1);
-      mbar_init(&sh->p_ready[i], 128);
-      mbar_init(&sh->pv_done[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh->s_full[i][b], 2);  // the scores, and what is said of them
+        mbar_init(&sh->p_ready[i][b], 128);
+        mbar_init(&sh->pv_done[i][b], 1);
+      }
       mbar_init(&sh->xchg[i], PAIR ? 256 : 128);
       mbar_init(&sh->drain[i], 1);
     }
@@ -521,63 +617,103 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int wk = PAIR ? 0 : warp >= 8 ? (warp - 8) >> 1 : warp >> 2;
   Walk w;
   bool more = w.start(p, sh->cut[wk], sh->cut[wk + 1].at);
+  constexpr int STEP = Cfg::STEP, AHEAD = Cfg::TILES;  // the scores run AHEAD steps before the values
 
   if (warp >= 8) {
     reg_dealloc<88>();
     uint8_t* ring = smem + Cfg::OFF_KV + wk * Cfg::SLOTS * Cfg::SLOT_BYTES;
     uint64_t* kv_full = sh->kv_full + wk * Cfg::SLOTS;
     uint64_t* kv_empty = sh->kv_empty + wk * Cfg::SLOTS;
+    int slot = 0;
     if ((warp & 1) != 0 && (!PAIR || warp == 9)) {
       // ------------------------------------------------------------ TMA warp
-      int slot = 0, seg = 0;
       uint32_t phase = 1;  // parity of the next kv_empty wait: the first round finds every slot free
-      int ld = 0;
+      int ld = 0, seg = 0;
       bool ok = true;
-      for (; more && ok; more = w.next(p), ++seg) {
-        if (!warp_wait(&sh->q_empty[wk], (seg & 1) ^ 1, ctx, SITE_ATTN_Q_EMPTY)) break;
-        if (lane == 0) {
-          constexpr int QT = PAIR ? 2 : 1;
-          mbar_arrive_expect_tx(&sh->q_full[wk], static_cast<uint32_t>(QT * Cfg::HALVES * p.tt * p.gp * 128));
-          for (int i = 0; i < QT; ++i)
-            for (int hf = 0; hf < Cfg::HALVES; ++hf)
-              tma_load_4d_at(&map_q, &sh->q_full[wk], smem + (wk + i) * Cfg::Q_BYTES + hf * (128 * 128), hf * 64, 0, w.h,
-                             w.s.q0 + w.t0(p, i));
+      const auto load = [&](const CUtensorMap* map, const Walk& at, int j, uint32_t info) {
+        const int kv_head = at.h * p.gp / p.group, key0 = j * STEP;
+        if (!(ok = warp_wait(&kv_empty[slot], phase, ctx, SITE_ATTN_KV_EMPTY))) return;
+        uint8_t* dst = ring + slot * Cfg::SLOT_BYTES;
+        int page = 0, key = 0;
+        const int rows = PAGED ? min(p.block_size, STEP) : STEP;
+        if constexpr (PAGED) {
+          // a lane per block; a block the table does not name is read out of range, as zeros
+          key = key0 + lane * rows;
+          page = -1;
+          const bool there = lane * rows < STEP && key < at.s.m;
+          if (there) page = p.table[at.b * p.ld_table + (key >> p.block_shift)];
+          const bool bad = page < 0 || page >= p.num_blocks;
+          if (bad) page = p.num_blocks;
+          info |= __ballot_sync(0xffffffffu, there && bad) << kInfoBad;
         }
-        const int kv_head = w.h * p.gp / p.group;
-        for (int j = w.j0; j < w.j1 && ok; ++j) {
-#pragma unroll 1
-          for (int x = 0; x < 2 * Cfg::SUBS && ok; ++x) {  // k, then v
-            const CUtensorMap* map = x < Cfg::SUBS ? &map_k : &map_v;
-            const int sub = x < Cfg::SUBS ? x : x - Cfg::SUBS;
-            const int key0 = j * kAttnStep + sub * Cfg::KEYS;
-            if (sub > 0 && key0 >= w.s.m) continue;        // nothing there
-            if (!(ok = warp_wait(&kv_empty[slot], phase, ctx, SITE_ATTN_KV_EMPTY))) break;
-            uint8_t* dst = ring + slot * Cfg::SLOT_BYTES;
-            if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], Cfg::SLOT_BYTES);
-            __syncwarp();
-            if constexpr (PAGED) {
-              // a lane per block; a block the table does not name is read out of range, as zeros
-              const int rows = min(p.block_size, Cfg::KEYS);
-              if (lane * rows < Cfg::KEYS) {
-                const int key = key0 + lane * rows;
-                int page = -1;
-                if (key < w.s.m) page = p.table[w.b * p.ld_table + (key >> p.block_shift)];
-                if (page < 0 || page >= p.num_blocks) page = p.num_blocks;
-                for (int hf = 0; hf < Cfg::HALVES; ++hf)
-                  tma_load_4d_at(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES + lane * rows * 128, hf * 64,
-                                 key & (p.block_size - 1), kv_head, page);
-              }
-            } else {
-              if (lane == 0)
-                for (int hf = 0; hf < Cfg::HALVES; ++hf)
-                  tma_load_3d(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES, hf * 64, kv_head, w.s.k0 + key0);
-            }
-            ++ld;
-            if (++slot == Cfg::SLOTS) {
-              slot = 0;
-              phase ^= 1;
-            }
+        if (lane == 0) {
+          sh->slot_info[wk * Cfg::SLOTS + slot] = info;
+          mbar_arrive_expect_tx(&kv_full[slot], Cfg::SLOT_BYTES);
+        }
+        __syncwarp();
+        if constexpr (PAGED) {
+          if (lane * rows < STEP)
+            for (int hf = 0; hf < Cfg::HALVES; ++hf)
+              tma_load_4d_at(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES + lane * rows * 128, hf * 64,
+                             key & (p.block_size - 1), kv_head, page);
+        } else {
+          if (lane == 0)
+            for (int hf = 0; hf < Cfg::HALVES; ++hf)
+              tma_load_3d(map, &kv_full[slot], dst + hf * Cfg::HALF_BYTES, hf * 64, kv_head, at.s.k0 + key0);
+        }
+        ++ld;
+        if (++slot == Cfg::SLOTS) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      // row tiles that step j counts for, and whether it begins or ends the segment
+      const auto about = [&](const Walk& at, int j, int st0, int st1) {
+        return (j < st0 ? kInfoRow0 : 0u) | (PAIR && j < st1 ? kInfoRow1 : 0u) | (j == at.j0 ? kInfoFirst : 0u) |
+               (j + 1 == at.j1 ? kInfoLast : 0u);
+      };
+      Walk wv = w;         // v follows k by AHEAD steps
+      int jk = w.j0, jv = w.j0;
+      int k0 = 0, k1 = 0, v0 = 0, v1 = 0;  // steps of the row tiles
+      if (more) {
+        k0 = v0 = w.row_steps(p, 0);
+        if (PAIR) k1 = v1 = w.row_steps(p, 1);
+      }
+      bool more_k = more;
+      for (int g = 0; more && ok; ++g) {
+        if (g >= AHEAD) {
+          const int valid = max(0, min(wv.s.m - jv * STEP, STEP));
+          load(&map_v, wv, jv, about(wv, jv, v0, v1) | static_cast<uint32_t>(valid) << kInfoValid);
+          if (++jv == wv.j1) {
+            more = wv.next(p);
+            jv = wv.j0;
+            v0 = wv.row_steps(p, 0);
+            if (PAIR) v1 = wv.row_steps(p, 1);
           }
+        }
+        if (ok && more_k) {
+          if (jk == w.j0) {
+            if (!(ok = warp_wait(&sh->q_empty[wk], (seg & 1) ^ 1, ctx, SITE_ATTN_Q_EMPTY))) break;
+            if (lane == 0) {
+              constexpr int QT = PAIR ? 2 : 1;
+              mbar_arrive_expect_tx(&sh->q_full[wk], static_cast<uint32_t>(QT * Cfg::HALVES * p.tt * p.gp * 128));
+              for (int i = 0; i < QT; ++i)
+                for (int hf = 0; hf < Cfg::HALVES; ++hf)
+                  tma_load_4d_at(&map_q, &sh->q_full[wk], smem + (wk + i) * Cfg::Q_BYTES + hf * (128 * 128), hf * 64, 0,
+                                 w.h, w.s.q0 + w.t0(p, i));
+            }
+            ++seg;
+          }
+          const uint32_t info = about(w, jk, k0, k1);
+          Walk now = w;
+          const int j = jk;
+          if (++jk == w.j1) {
+            more_k = w.next(p);
+            jk = w.j0;
+            k0 = w.row_steps(p, 0);
+            if (PAIR) k1 = w.row_steps(p, 1);
+          }
+          load(&map_k, now, j, info | (more_k ? 0u : kInfoEnd));
         }
       }
       // every load in flight has landed before the CTA ends
@@ -589,151 +725,95 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (seg > 0) mbar_wait(&sh->q_full[wk], static_cast<uint32_t>((seg - 1) & 1), ctx, SITE_ATTN_DRAIN, false);
     } else if ((warp & 1) == 0 && (!PAIR || warp == 8)) {
       // ------------------------------------------------------------ MMA warp
-      constexpr int G0 = 0, GN = PAIR ? 2 : 1;  // row tiles this warp serves
-      constexpr uint32_t idesc_s = make_idesc_16bit(128, Cfg::KEYS, F16);
+      // One warp issues for both row tiles, tile by tile: issued by two warps
+      // the products of the tiles take turns on the tensor pipe, both groups
+      // get their scores at the same time and both want the exponential unit
+      // at the same time (measured: 2200 cycles for 128 keys instead of 1150).
+      constexpr int GN = PAIR ? 2 : 1;         // row tiles
+      constexpr uint32_t idesc_s = make_idesc_16bit(128, STEP, F16);
       constexpr uint32_t idesc_o = make_idesc_16bit(128, D, F16) | kIdescBMnMajor;
-      int slot = 0, seg = 0;
-      uint32_t phase = 0;
-      int n_p[GN] = {};  // probability tiles consumed, per row tile
+      const uint64_t q_desc = make_sw128_desc(smem_addr(smem + wk * Cfg::Q_BYTES));
+      const uint64_t k_desc = make_sw128_desc(smem_addr(ring));
+      const uint64_t v_desc = make_sw128_mn_desc(smem_addr(ring), Cfg::HALF_BYTES);
+      const volatile uint32_t* slot_info = sh->slot_info + wk * Cfg::SLOTS;
+      uint32_t phase = 0, q_phase = 0;
+      unsigned n_q[GN] = {}, n_p[GN] = {};     // score and probability tiles so far
       bool ok = true;
-      // the next slot of the ring, in the order of the loads
-      const auto take = [&]() -> int {
-        if (!(ok = warp_wait(&kv_full[slot], phase, ctx, SITE_ATTN_KV_FULL))) return slot;
+      // waits for the next slot of the ring, in the order of the loads
+      const auto take = [&](uint32_t* info) -> int {
+        ok = ok && warp_wait(&kv_full[slot], phase, ctx, SITE_ATTN_KV_FULL);
         const int got = slot;
+        *info = slot_info[got];
         if (++slot == Cfg::SLOTS) {
           slot = 0;
           phase ^= 1;
         }
         return got;
       };
-      const auto release = [&](int sl) {
-        if (lane == 0) umma_commit(&kv_empty[sl]);
-      };
-      const auto scores = [&](int i, int sl, int sub) {  // S_i = Q_i K^T, the columns of one slot
-        if (lane == 0) {
-          const uint32_t a = smem_addr(smem + (wk + i) * Cfg::Q_BYTES);
-          const uint32_t bk = smem_addr(ring + sl * Cfg::SLOT_BYTES);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16kind(tmem + (wk + i) * 128 + sub * Cfg::KEYS,
-                         make_sw128_desc(a + (k / 4) * (128 * 128) + (k % 4) * 32),
-                         make_sw128_desc(bk + (k / 4) * Cfg::HALF_BYTES + (k % 4) * 32), idesc_s, k > 0);
+      int stop = more ? INT_MAX : 0;           // known once the last k has come
+      for (int g = 0; g < stop; ++g) {
+        const bool do_v = g >= AHEAD, do_k = stop == INT_MAX;
+        uint32_t iv = 0, ik = 0;
+        int sv = 0, sk = 0;
+        if (do_v) {
+          sv = take(&iv);
+          const int valid = iv >> kInfoValid & 0xff;
+          if (ok && valid < STEP) {
+            // rows behind the last key are other requests' or nobody's: zeros
+            uint8_t* t = ring + sv * Cfg::SLOT_BYTES;
+            for (int x = valid * 8 + lane; x < STEP * 8; x += 32)
+              for (int hf = 0; hf < Cfg::HALVES; ++hf)
+                *reinterpret_cast<uint4*>(t + hf * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
         }
-      };
-      const auto values = [&](int i, int sl, int sub, bool first) {  // O_i (+)= P_i V
-        if (lane == 0) {
-          const uint32_t bv = smem_addr(ring + sl * Cfg::SLOT_BYTES);
-#pragma unroll
-          for (int k = 0; k < Cfg::KEYS / 16; ++k)
-            umma_f16kind_ts(tmem + 256 + (wk + i) * D, tmem + (wk + i) * 128 + (sub * (Cfg::KEYS / 16) + k) * 8,
-                            make_sw128_mn_desc(bv + k * 2048, Cfg::HALF_BYTES), idesc_o, !first || k > 0);
+        if (do_k) {
+          sk = take(&ik);
+          if ((ik & kInfoEnd) != 0) stop = g + 1 + AHEAD;
+          if ((ik & kInfoFirst) != 0) {
+            ok = ok && warp_wait(&sh->q_full[wk], q_phase, ctx, SITE_ATTN_Q);
+            q_phase ^= 1;
+          }
         }
-      };
-      // v rows behind the last key are other requests' or nobody's: zeros
-      const auto clean = [&](int sl, int key0) {
-        const int valid = w.s.m - key0;
-        if (valid < Cfg::KEYS) {
-          uint8_t* t = ring + sl * Cfg::SLOT_BYTES;
-          for (int x = max(valid, 0) * 8 + lane; x < Cfg::KEYS * 8; x += 32)
-            for (int hf = 0; hf < Cfg::HALVES; ++hf)
-              *reinterpret_cast<uint4*>(t + hf * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      };
-      // slots of step j that were loaded
-      const auto subs_of = [&](int j) {
-        int n = 1;
-        while (n < Cfg::SUBS && j * kAttnStep + n * Cfg::KEYS < w.s.m) ++n;
-        return n;
-      };
-      for (; more && ok; more = w.next(p), ++seg) {
-        int st[GN];
-        bool started[GN] = {};
 #pragma unroll
-        for (int i = 0; i < GN; ++i) st[i] = w.row_steps(p, i);
-        if (!(ok = warp_wait(&sh->q_full[wk], seg & 1, ctx, SITE_ATTN_Q))) break;
-        for (int j = w.j0; j <= w.j1 && ok; ++j) {
-          // v of step j - 1 and k of step j, row tile by row tile
-          const bool do_v = j > w.j0, do_k = j < w.j1;
-          int sv[Cfg::SUBS], sk[Cfg::SUBS];
-          const int nv = do_v ? subs_of(j - 1) : 0, nk = do_k ? subs_of(j) : 0;
-          bool have_v = false, have_k = false;
+        for (int x = 0; x < GN; ++x) {
+          const int i = wk + x;                // group
+          const uint32_t mine = x == 0 ? kInfoRow0 : kInfoRow1;
+          const uint32_t t_s = tmem + i * 128, t_o = tmem + 256 + i * D;
+          if ((iv & mine) != 0) {              // O (+)= P V, 64 keys at a time
 #pragma unroll
-          for (int i = G0; i < GN; ++i) {
-            if (ok && do_v && j - 1 < st[i]) {
-              ok = warp_wait(&sh->p_ready[wk + i], n_p[i] & 1, ctx, SITE_ATTN_P);
-              ++n_p[i];
-              if (!have_v) {
-#pragma unroll
-                for (int x = 0; x < Cfg::SUBS; ++x)
-                  if (ok && x < nv) {
-                    sv[x] = take();
-                    if (ok) clean(sv[x], (j - 1) * kAttnStep + x * Cfg::KEYS);
-                  }
-                have_v = true;
-              }
-              if (ok) {
-                tc_fence_after();
-#pragma unroll
-                for (int x = 0; x < Cfg::SUBS; ++x)
-                  if (x < nv) values(i, sv[x], x, !started[i] && x == 0);
-                started[i] = true;
-                if (lane == 0) umma_commit(&sh->pv_done[wk + i]);
-                if (!PAIR) {
-#pragma unroll
-                  for (int x = 0; x < Cfg::SUBS; ++x)
-                    if (x < nv) release(sv[x]);
-                }
-              }
+            for (int hf = 0; hf < STEP / 64; ++hf) {
+              // one barrier per 64 probabilities: the halves of a tile, or the two tiles in turn
+              const int b = PAIR ? hf : n_p[x] & 1;
+              ok = ok && warp_wait(&sh->p_ready[i][b], PAIR ? n_p[x] & 1 : n_p[x] >> 1 & 1, ctx, SITE_ATTN_P);
+              if (!ok) break;
+              tc_fence_after();
+              umma_values(t_o, t_s + b * (PAIR ? 32 : 64), v_desc + (sv * Cfg::SLOT_BYTES + hf * 64 * 128) / 16, idesc_o,
+                          hf > 0 || (iv & kInfoFirst) == 0);
             }
-            if (ok && do_k && j < st[i]) {
-              if (!have_v && do_v) {  // the ring is taken in order
-#pragma unroll
-                for (int x = 0; x < Cfg::SUBS; ++x)
-                  if (ok && x < nv) sv[x] = take();
-                have_v = true;
-              }
-              if (!have_k) {
-#pragma unroll
-                for (int x = 0; x < Cfg::SUBS; ++x)
-                  if (ok && x < nk) sk[x] = take();
-                have_k = true;
-              }
-              if (ok) {
-                tc_fence_after();
-#pragma unroll
-                for (int x = 0; x < Cfg::SUBS; ++x)
-                  if (x < nk) {
-                    scores(i, sk[x], x);
-                    if (!PAIR) release(sk[x]);
-                  }
-                if (lane == 0) umma_commit(&sh->s_full[wk + i]);
-              }
+            if (ok) umma_commit_elected(&sh->pv_done[i][PAIR ? 0 : n_p[x] & 1]);
+            ++n_p[x];
+          }
+          if (ok && (ik & mine) != 0) {        // S = Q K^T
+            const int b = PAIR ? 0 : n_q[x] & 1;
+            tc_fence_after();
+            umma_scores<D / 16, Cfg::HALF_BYTES>(t_s + b * 64, q_desc + x * (Cfg::Q_BYTES / 16),
+                                                 k_desc + sk * (Cfg::SLOT_BYTES / 16), idesc_s);
+            umma_commit_elected(&sh->s_full[i][b]);
+            if (lane == 0) {
+              sh->score_info[i][b] = ik;
+              mbar_arrive(&sh->s_full[i][b]);
             }
+            ++n_q[x];
           }
-          // tiles that nothing used have landed before their slots are handed back
-          if (ok && do_v && !have_v) {
-#pragma unroll
-            for (int x = 0; x < Cfg::SUBS; ++x)
-              if (ok && x < nv) sv[x] = take();
-          }
-          if (ok && do_k && !have_k) {
-#pragma unroll
-            for (int x = 0; x < Cfg::SUBS; ++x)
-              if (ok && x < nk) sk[x] = take();
-          }
-          if (!ok) break;
-          const bool spare_v = PAIR || !have_v, spare_k = PAIR || !have_k;
-#pragma unroll
-          for (int x = 0; x < Cfg::SUBS; ++x) {
-            if (spare_v && x < nv) release(sv[x]);
-            if (spare_k && x < nk) release(sk[x]);
-          }
-          if (j == w.j1 - 1 && lane == 0) umma_commit(&sh->q_empty[wk]);  // the last product with q is issued
         }
+        if (!ok) break;
+        if (do_v) umma_commit_elected(&kv_empty[sv]);
+        if (do_k) umma_commit_elected(&kv_empty[sk]);
+        if ((ik & kInfoLast) != 0) umma_commit_elected(&sh->q_empty[wk]);  // the last product with this q is issued
       }
-      if (lane == 0) umma_commit(&sh->drain[wk]);
+      umma_commit_elected(&sh->drain[wk]);
       __syncwarp();
       mbar_wait(&sh->drain[wk], 0, ctx, SITE_ATTN_DRAIN, false);
     }
@@ -748,7 +828,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + i * 128, t_o = tmem + lanes + 256 + i * D;
     const int row_token = r / p.gp, row_head = r - row_token * p.gp;
-    int n_s = 0, n_x = 0;                             // score tiles taken; exchanges
+    unsigned n_s = 0, n_x = 0;                        // score tiles taken; exchanges
     bool ok = true;
     const auto meet = [&]() {                         // all threads of the worker
       mbar_arrive(&sh->xchg[wk]);
@@ -770,38 +850,32 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       bool some = false;
       const int last_j = min(w.j1, steps_i);
       for (int j = w.j0; j < last_j; ++j) {
-        unsigned bad_pages = 0;
-        if constexpr (PAGED) {
-          const int rows = min(p.block_size, kAttnStep);
-          const int key = j * kAttnStep + lane * rows;
-          bool bad = false;
-          if (lane * rows < kAttnStep && key < w.s.m) {
-            const int page = p.table[w.b * p.ld_table + (key >> p.block_shift)];
-            bad = page < 0 || page >= p.num_blocks;
-          }
-          bad_pages = __ballot_sync(0xffffffffu, bad);
-        }
-        if (!(ok = warp_wait(&sh->s_full[i], n_s & 1, ctx, SITE_ATTN_S))) break;
+        const int sb = PAIR ? 0 : n_s & 1;
+        if (!(ok = warp_wait(&sh->s_full[i][sb], (PAIR ? n_s : n_s >> 1) & 1, ctx, SITE_ATTN_S))) break;
         if (!warp_ok) {                               // rows of nobody: their probabilities stay what they are
-          mbar_arrive(&sh->p_ready[i]);
+          mbar_arrive(&sh->p_ready[i][sb]);
+          if (PAIR) mbar_arrive(&sh->p_ready[i][1]);
           ++n_s;
           continue;
         }
         tc_fence_after();
-        float s[128];
+        const uint32_t t_sb = t_s + sb * 64;
+        float s[STEP];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld_x32(t_s + x * 32, reinterpret_cast<uint32_t(&)[32]>(s[x * 32]));
+        for (int x = 0; x < STEP; x += 32) tmem_ld_x32(t_sb + x, reinterpret_cast<uint32_t(&)[32]>(s[x]));
         tmem_ld_wait();
         if (p.neg) {
 #pragma unroll
-          for (int x = 0; x < 128; ++x) s[x] = -s[x];
+          for (int x = 0; x < STEP; ++x) s[x] = -s[x];
         }
-        const int rel = j * kAttnStep;
-        if (rel + kAttnStep > open || bad_pages != 0) {
+        const int rel = j * STEP;
+        unsigned bad_pages = 0;
+        if constexpr (PAGED) bad_pages = *const_cast<volatile uint32_t*>(&sh->score_info[i][sb]) >> kInfoBad;
+        if (rel + STEP > open || bad_pages != 0) {
           // one bit per key of the step
-          uint32_t vis[4];
+          uint32_t vis[STEP / 32];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < STEP / 32; ++x) {
             const int lim = sees - rel - 32 * x;
             vis[x] = lim >= 32 ? 0xffffffffu : lim > 0 ? (1u << lim) - 1u : 0u;
           }
@@ -809,7 +883,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             // the tree's 64 bits, moved to where its first key lies in this step
             const int at = w.s.first - rel;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
+            for (int x = 0; x < STEP / 32; ++x) {
               const int by = at - 32 * x;             // bit 0 of the tree in this word's coordinates
               uint32_t part = 0;
               if (by > -64 && by < 32) part = by >= 0 ? static_cast<uint32_t>(bits << by) : static_cast<uint32_t>(bits >> -by);
@@ -819,27 +893,28 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
           }
           if constexpr (PAGED) {
-            const int rows = min(p.block_size, kAttnStep);
+            const int rows = min(p.block_size, STEP);
             for (unsigned rest = bad_pages; rest != 0; rest &= rest - 1) {
               const int lo = (__ffs(rest) - 1) * rows;
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
+              for (int x = 0; x < STEP / 32; ++x) {
                 const int a = max(lo - 32 * x, 0), z = min(lo + rows - 32 * x, 32);
                 if (a < z) vis[x] &= ~((z - a == 32 ? 0xffffffffu : (1u << (z - a)) - 1u) << a);
               }
             }
           }
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
+          for (int x = 0; x < STEP; ++x)
             if (!(vis[x / 32] >> (x % 32) & 1u)) s[x] = -INFINITY;
         }
-        float top = fmaxf(s[0], s[1]), top2 = fmaxf(s[2], s[3]);
+        float tops[4] = {s[0], s[1], s[2], s[3]};     // independent chains
 #pragma unroll
-        for (int x = 4; x < 128; x += 4) {
-          top = fmaxf(top, fmaxf(s[x], s[x + 1]));
-          top2 = fmaxf(top2, fmaxf(s[x + 2], s[x + 3]));
+        for (int x = 4; x < STEP; x += 8) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            tops[y] = x + 4 < STEP ? fmaxf(tops[y], fmaxf(s[x + y], s[x + 4 + y])) : fmaxf(tops[y], s[x + y]);
         }
-        top = fmaxf(top, top2);
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         // a new base only where the maximum has grown by more than the stale one absorbs
         const bool grow = top > m && (m == -INFINITY || (top - m) * p.c > kAttnLazy);
         if (__any_sync(0xffffffffu, grow)) {
@@ -849,7 +924,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             l *= alpha;
           }
           if (some) {
-            if (!(ok = warp_wait(&sh->pv_done[i], (n_s - 1) & 1, ctx, SITE_ATTN_PV))) break;
+            const unsigned last = n_s - 1;
+            if (!(ok = warp_wait(&sh->pv_done[i][PAIR ? 0 : last & 1], (PAIR ? last : last >> 1) & 1, ctx, SITE_ATTN_PV)))
+              break;
             tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < D; x += 32) {
@@ -863,32 +940,34 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             tmem_st_wait();
           }
         }
-        const float base = m == -INFINITY ? 0.f : m * p.c;
-        float sum0 = 0.f, sum1 = 0.f;
+        const float neg_base = m == -INFINITY ? 0.f : -m * p.c;
+        float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < STEP / 64; ++hf) {
           uint32_t pk[32];
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
-            const float a = exp2_approx(fmaf(s[hf * 64 + 2 * x], p.c, -base));
-            const float b = exp2_approx(fmaf(s[hf * 64 + 2 * x + 1], p.c, -base));
-            sum0 += a;
-            sum1 += b;
-            pk[x] = pack_pair<T>(a, b);
+            float2 e = fma2(make_float2(s[hf * 64 + 2 * x], s[hf * 64 + 2 * x + 1]), make_float2(p.c, p.c),
+                            make_float2(neg_base, neg_base));
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
+            sums = add2(sums, e);
+            pk[x] = pack_pair<T>(e.x, e.y);
           }
-          tmem_st_x32(t_s + hf * 32, pk);
+          tmem_st_x32(t_sb + hf * 32, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&sh->p_ready[i][PAIR ? hf : sb]);
         }
-        l += sum0 + sum1;
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&sh->p_ready[i]);
+        l += sums.x + sums.y;
         ++n_s;
         some = true;
       }
       ok = __all_sync(0xffffffffu, ok && *ctx.abort_flag == 0);
       if (!ok) break;
       if (some) {
-        if (!(ok = warp_wait(&sh->pv_done[i], (n_s - 1) & 1, ctx, SITE_ATTN_PV))) break;
+        const unsigned last = n_s - 1;
+        if (!(ok = warp_wait(&sh->pv_done[i][PAIR ? 0 : last & 1], (PAIR ? last : last >> 1) & 1, ctx, SITE_ATTN_PV))) break;
         tc_fence_after();
       }
       // ---------------------------------------------------- the segment's end
@@ -905,31 +984,39 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float probe = 0.f;                            // NaN when any output is not finite
 #pragma unroll 1
         for (int x = 0; x < D; x += 32) {
-          float v[32];
-          tmem_ld_x32(t_o + x, reinterpret_cast<uint32_t(&)[32]>(v));
+          uint32_t v[32];
+          tmem_ld_x32(t_o + x, v);
           tmem_ld_wait();
           if (!some) {
 #pragma unroll
-            for (int y = 0; y < 32; ++y) v[y] = 0.f;
+            for (int y = 0; y < 32; ++y) v[y] = 0;
           }
 #pragma unroll
-          for (int y = 0; y < 32; ++y) probe = fmaf(v[y], 0.f, probe);
+          for (int y = 0; y < 32; ++y) probe = fmaf(__uint_as_float(v[y]), 0.f, probe);
           if (row_ok) {
             if (whole) {
 #pragma unroll
-              for (int y = 0; y < 32; y += 8) {
-                uint4 o;
-                o.x = pack_pair<T>(v[y] * inv, v[y + 1] * inv);
-                o.y = pack_pair<T>(v[y + 2] * inv, v[y + 3] * inv);
-                o.z = pack_pair<T>(v[y + 4] * inv, v[y + 5] * inv);
-                o.w = pack_pair<T>(v[y + 6] * inv, v[y + 7] * inv);
-                *reinterpret_cast<uint4*>(dst + x + y) = o;
+              for (int y = 0; y < 32; y += 16) {
+                uint32_t o[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z)
+                  o[z] = pack_pair<T>(__uint_as_float(v[y + 2 * z]) * inv, __uint_as_float(v[y + 2 * z + 1]) * inv);
+                store_32(dst + x + y, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], p.wide);
               }
             } else {
 #pragma unroll
-              for (int y = 0; y < 32; y += 4)
-                __stcg(reinterpret_cast<float4*>(part) + ((x + y) >> 2) * Cfg::PART_ROWS + row,
-                       make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]));
+              for (int y = 0; y < 32; y += 8) {
+                if constexpr (PAIR) {  // [element / 4][row][4]: many rows, a warp writes whole lines
+                  float4* at = reinterpret_cast<float4*>(part) + (x + y) / 4 * Cfg::PART_ROWS + row;
+                  __stcg(at, make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]), __uint_as_float(v[y + 2]),
+                                         __uint_as_float(v[y + 3])));
+                  __stcg(at + Cfg::PART_ROWS, make_float4(__uint_as_float(v[y + 4]), __uint_as_float(v[y + 5]),
+                                                          __uint_as_float(v[y + 6]), __uint_as_float(v[y + 7])));
+                } else {               // [row][element]: few rows, a warp reads whole rows
+                  store_32(part + row * D + x + y, v[y], v[y + 1], v[y + 2], v[y + 3], v[y + 4], v[y + 5], v[y + 6],
+                           v[y + 7], true);
+                }
+              }
             }
           }
         }
@@ -946,7 +1033,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int rw = __shfl_sync(0xffffffffu, row, src);
           const float bs = __shfl_sync(0xffffffffu, base, src), iv = __shfl_sync(0xffffffffu, inv, src);
           float o[D / 32];
-          attn_row<T, D>(p, w.s, w.b, tk, hd, kv_head, w.j0 * kAttnStep, min(w.j1 * kAttnStep, w.s.m), bs, o);
+          attn_row<T, D>(p, w.s, w.b, tk, hd, kv_head, w.j0 * STEP, min(w.j1 * STEP, w.s.m), bs, o);
           __syncwarp();
 #pragma unroll
           for (int e = 0; e < D / 32; ++e) {
@@ -955,19 +1042,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               static_cast<T*>(p.out)[static_cast<long long>(w.s.q0 + tk) * p.out_token + hd * p.out_head + d] =
                   elem_from_float<T>(o[e] * iv);
             else
-              __stcg(part + ((d >> 2) * Cfg::PART_ROWS + rw) * 4 + (d & 3), o[e]);
+              __stcg(part + (PAIR ? (d / 4 * Cfg::PART_ROWS + rw) * 4 + d % 4 : rw * D + d), o[e]);
           }
         }
       }
       tc_fence_before();
       if (!whole) {
         // the last worker of the unit to arrive joins the partials, in the order of the keys
-        __threadfence();
         if (!(ok = meet())) break;
-        const long long unit0 = w.at - w.j0;
-        const int c0 = static_cast<int>(quotient(unit0, sh->per));
-        const int c1 = static_cast<int>(quotient(unit0 + w.steps - 1, sh->per));
+        const long long unit0 = w.at - (w.j0 == 0 ? 0 : kUnitCost + w.j0);
+        const int c0 = static_cast<int>(quotient(unit0 + kUnitCost, sh->per));
+        const int c1 = static_cast<int>(quotient(unit0 + kUnitCost + w.steps - 1, sh->per));
         if (gtid == 0) {
+          __threadfence();
           const int arrived = atom_add_acq_rel_gpu(&p.counters[c0], 1);
           sh->last[wk] = arrived == c1 - c0;
           if (arrived == c1 - c0) p.counters[c0] = 0;
@@ -983,86 +1070,128 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           float* jm = sh->m + wk * 128;
           float* jl = sh->l + wk * 128;
           // per row: the common maximum and 1 / sum
-          if (rows <= 32) {
-            for (int x = gtid >> 5; x < rows; x += GT / 32) {  // a warp per row, lanes over the partials
+          const float* stats = p.partials + Cfg::PART_ROWS * D;
+          const auto stat = [&](int c) { return stats + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS; };
+          if (!PAIR && rows <= 16) {                  // a warp per row, lanes over the partials
+            for (int x = gtid >> 5; x < rows; x += GT / 32) {
               float mm = -INFINITY, ll = 0.f;
-              for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(partial(c) + Cfg::PART_ROWS * D + x));
-              for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-              if (mm == -INFINITY) mm = 0.f;
-              for (int c = c0 + lane; c <= c1; c += 32)
-                ll += exp2_approx(__ldcg(partial(c) + Cfg::PART_ROWS * D + x) - mm) *
-                      __ldcg(partial(c) + Cfg::PART_ROWS * (D + 1) + x);
-              for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+              for (int b0 = c0; b0 <= c1; b0 += 32) {
+                const int c = b0 + lane;
+                const float mv = c <= c1 ? __ldcg(stat(c) + x) : -INFINITY;
+                const float lv = c <= c1 ? __ldcg(stat(c) + Cfg::PART_ROWS + x) : 0.f;
+                float top = fmaxf(mm, mv);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float safe = top == -INFINITY ? 0.f : top;
+                float sum = exp2_approx(mv - safe) * lv;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                ll = ll * exp2_approx(mm - safe) + sum;
+                mm = top;
+              }
               if (lane == 0) {
-                jm[x] = mm;
+                jm[x] = mm == -INFINITY ? 0.f : mm;
                 jl[x] = ll == 0.f ? 0.f : 1.f / ll;
               }
             }
-          } else {
-            const int x = gtid;                       // a thread per row
-            if (x < rows0 || (x >= 128 && x - 128 < rows - rows0)) {
-              float mm = -INFINITY, ll = 0.f;
+          } else if (gtid < rows0 || (PAIR && gtid >= 128 && gtid - 128 < rows - rows0)) {  // a thread per row
+            float mm = -INFINITY, ll = 0.f;
 #pragma unroll 4
-              for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(partial(c) + Cfg::PART_ROWS * D + x));
-              if (mm == -INFINITY) mm = 0.f;
+            for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(stat(c) + gtid));
+            if (mm == -INFINITY) mm = 0.f;
 #pragma unroll 4
-              for (int c = c0; c <= c1; ++c)
-                ll += exp2_approx(__ldcg(partial(c) + Cfg::PART_ROWS * D + x) - mm) *
-                      __ldcg(partial(c) + Cfg::PART_ROWS * (D + 1) + x);
-              jm[x] = mm;
-              jl[x] = ll == 0.f ? 0.f : 1.f / ll;
-            }
+            for (int c = c0; c <= c1; ++c)
+              ll += exp2_approx(__ldcg(stat(c) + gtid) - mm) * __ldcg(stat(c) + Cfg::PART_ROWS + gtid);
+            jm[gtid] = mm;
+            jl[gtid] = ll == 0.f ? 0.f : 1.f / ll;
           }
           if (!(ok = meet())) break;
-          const int items = rows * (D / 4);
-          constexpr int U = 4;
-          for (int it0 = gtid; it0 < items; it0 += GT * U) {
-            float4 acc[U];
-            int rowu[U], du[U];
-            float mu[U];
+          if constexpr (PAIR) {
+            // a thread per row, 32 elements at a time
+            if (gtid < rows0 || (gtid >= 128 && gtid - 128 < rows - rows0)) {
+              const float mm = jm[gtid], iv = jl[gtid];
+#pragma unroll 1
+              for (int x = 0; x < D; x += 32) {
+                float acc[32];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int it = min(it0 + GT * u, items - 1);
-              du[u] = it / rows;
-              const int x = it - du[u] * rows;
-              rowu[u] = x < rows0 ? x : 128 + x - rows0;
-              mu[u] = jm[rowu[u]];
-              acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+                for (int y = 0; y < 32; ++y) acc[y] = 0.f;
 #pragma unroll 2
-            for (int c = c0; c <= c1; ++c) {
-              const float* sl = partial(c);
-              float wt[U];
-              float4 o[U];
+                for (int c = c0; c <= c1; ++c) {
+                  const float f = exp2_approx(__ldcg(stat(c) + gtid) - mm);
+                  const float4* from = reinterpret_cast<const float4*>(partial(c)) + x / 4 * Cfg::PART_ROWS + gtid;
 #pragma unroll
-              for (int u = 0; u < U; ++u) {
-                wt[u] = __ldcg(sl + Cfg::PART_ROWS * D + rowu[u]);
-                o[u] = __ldcg(reinterpret_cast<const float4*>(sl) + du[u] * Cfg::PART_ROWS + rowu[u]);
-              }
+                  for (int y = 0; y < 8; ++y) {
+                    const float4 o = __ldcg(from + y * Cfg::PART_ROWS);
+                    acc[4 * y] = fmaf(f, o.x, acc[4 * y]);
+                    acc[4 * y + 1] = fmaf(f, o.y, acc[4 * y + 1]);
+                    acc[4 * y + 2] = fmaf(f, o.z, acc[4 * y + 2]);
+                    acc[4 * y + 3] = fmaf(f, o.w, acc[4 * y + 3]);
+                  }
+                }
 #pragma unroll
-              for (int u = 0; u < U; ++u) {
-                const float f = exp2_approx(wt[u] - mu[u]);
-                acc[u].x = fmaf(f, o[u].x, acc[u].x);
-                acc[u].y = fmaf(f, o[u].y, acc[u].y);
-                acc[u].z = fmaf(f, o[u].z, acc[u].z);
-                acc[u].w = fmaf(f, o[u].w, acc[u].w);
-              }
-            }
+                for (int y = 0; y < 32; y += 16) {
+                  uint32_t o[8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              if (it0 + GT * u < items) {
-                const int rr = rowu[u] & 127;
-                const float iv = jl[rowu[u]];
-                const int tk = w.t0(p, rowu[u] >> 7) + rr / p.gp, hd = w.h * p.gp + rr % p.gp;
-                uint2 o;
-                o.x = pack_pair<T>(acc[u].x * iv, acc[u].y * iv);
-                o.y = pack_pair<T>(acc[u].z * iv, acc[u].w * iv);
-                *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<long long>(w.s.q0 + tk) * p.out_token +
-                                          hd * p.out_head + du[u] * 4) = o;
+                  for (int z = 0; z < 8; ++z) o[z] = pack_pair<T>(acc[y + 2 * z] * iv, acc[y + 2 * z + 1] * iv);
+                  store_32(dst + x + y, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], p.wide);
+                }
               }
             }
+          } else {
+            // a warp per row (two at head_dim 64), U rows and C partials at a time
+            constexpr int LANES = D / 4, PER = 32 / LANES;
+            const int sub = lane / LANES, d4 = lane % LANES;
+            const auto join = [&](auto u_, auto c_) {
+              constexpr int U = decltype(u_)::value, C = decltype(c_)::value;
+              for (int x0 = (gtid >> 5) * PER + sub; x0 < rows; x0 += GT / 32 * PER * U) {
+                float4 acc[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int b0 = c0; b0 <= c1; b0 += C) {
+                  float4 o[U][C];
+                  float f[U][C];
+#pragma unroll
+                  for (int k = 0; k < C; ++k) {
+                    const int c = min(b0 + k, c1);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                      const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
+                      o[u][k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
+                      f[u][k] = __ldcg(stat(c) + x);
+                    }
+                  }
+#pragma unroll
+                  for (int k = 0; k < C; ++k) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                      const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
+                      const float e = b0 + k <= c1 ? exp2_approx(f[u][k] - jm[x]) : 0.f;
+                      acc[u].x = fmaf(e, o[u][k].x, acc[u].x);
+                      acc[u].y = fmaf(e, o[u][k].y, acc[u].y);
+                      acc[u].z = fmaf(e, o[u][k].z, acc[u].z);
+                      acc[u].w = fmaf(e, o[u][k].w, acc[u].w);
+                    }
+                  }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                  const int x = x0 + u * (GT / 32 * PER);
+                  if (x < rows) {
+                    const float iv = jl[x];
+                    const int tk = w.t0(p, 0) + x / p.gp, hd = w.h * p.gp + x % p.gp;
+                    uint2 o;
+                    o.x = pack_pair<T>(acc[u].x * iv, acc[u].y * iv);
+                    o.y = pack_pair<T>(acc[u].z * iv, acc[u].w * iv);
+                    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<long long>(w.s.q0 + tk) * p.out_token +
+                                              hd * p.out_head + d4 * 4) = o;
+                  }
+                }
+              }
+            };
+            if (rows <= GT / 32 * PER) join(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+            else join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
           }
-          if (!(ok = meet())) break;
+          if (!(ok = meet())) break;  // jm and jl may be written again
         }
       }
     }
