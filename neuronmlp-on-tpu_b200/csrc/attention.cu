@@ -8,6 +8,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <utility>
 
 #include "../../include/svdmlp.h"
 #include "attention_sm100.cuh"
@@ -25,14 +26,31 @@ static bool rows_aligned(const void* p, int64_t token, int64_t head) {
 
 static bool elems_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
+// A launch that may overlap the previous kernel on the stream: each of these
+// kernels waits on the device (griddepcontrol.wait) before it reads or writes
+// anything, and lets its own successor launch at once.
+template <typename... Params, typename... Args>
+static int launch_overlapped(void (*kernel)(Params...), int grid, int threads, size_t smem, cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SVD_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+  count_launch();
+  return SVDMLP_OK;
+}
+
 // --------------------------------------------------------------------- rope
 template <typename T, int E>
 static int launch_rope(const RopeParams& p, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((p.tokens + p.tile - 1) / p.tile);
-  rope_kernel<T, E><<<grid, kRopeThreads, static_cast<size_t>(p.tile) * p.half * sizeof(float2), s>>>(p);
-  SVD_CUDA(cudaGetLastError());
-  count_launch();
-  return SVDMLP_OK;
+  return launch_overlapped(rope_kernel<T, E>, (p.tokens + p.tile - 1) / p.tile, kRopeThreads,
+                           static_cast<size_t>(p.tile) * p.half * sizeof(float2), s, p);
 }
 
 static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
@@ -123,10 +141,7 @@ static int pages_impl(const svdmlp_pages_args* a, cudaStream_t s) {
   p.count_out = a->count_out;
   p.missing = a->missing;
   const int grid = std::max(1, std::min(planning_sms(), (a->tokens + kPagesThreads - 1) / kPagesThreads));
-  page_step_kernel<<<static_cast<unsigned>(grid), kPagesThreads, 0, s>>>(p);
-  SVD_CUDA(cudaGetLastError());
-  count_launch();
-  return SVDMLP_OK;
+  return launch_overlapped(page_step_kernel, grid, kPagesThreads, 0, s, p);
 }
 
 // ---------------------------------------------------------------- attention
@@ -187,10 +202,7 @@ static int launch_attention(const CUtensorMap& q, const CUtensorMap& k, const CU
     SVD_CUDA(cudaFuncSetAttribute(attention_kernel<T, D, PAGED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  attention_kernel<T, D, PAGED, PAIR><<<static_cast<unsigned>(grid), kAttnThreads, SMEM, s>>>(q, k, v, p);
-  SVD_CUDA(cudaGetLastError());
-  count_launch();
-  return SVDMLP_OK;
+  return launch_overlapped(attention_kernel<T, D, PAGED, PAIR>, grid, kAttnThreads, SMEM, s, q, k, v, p);
 }
 
 template <bool PAGED, bool PAIR>
@@ -218,7 +230,6 @@ static void common_params(AttnParams* p, const Args* a, int q_tokens) {
   // a zero scale would turn masked scores (-inf) into NaN; the smallest one gives the same weights
   p->c = std::max(std::fabs(a->scale) * 1.4426950408889634f, 1e-30f);
   p->neg = a->scale < 0;
-  p->wide = (reinterpret_cast<uintptr_t>(a->out) & 31u) == 0 && a->out_token % 16 == 0 && a->out_head % 16 == 0;
   p->cu_q = a->cu_q;
   p->q = a->q;
   p->q_token = a->q_token;
@@ -233,9 +244,15 @@ static void common_params(AttnParams* p, const Args* a, int q_tokens) {
   p->timeout_ns = wait_limit_ns();
 }
 
-static int attn_grid(int* grid) {
+// One CTA per SM, or fewer where there cannot be work for all: at most `tokens`
+// rows in `batch` requests, of at most `keys` keys each.
+static int attn_grid(const AttnParams& p, bool pair, int64_t tokens, int64_t keys, int* grid) {
   SVD_CHECK(device_sms(grid));
   *grid = std::min(*grid, kAttnMaxGrid);
+  const int64_t units = (tokens / (pair ? 2 * p.tt : p.tt) + p.batch) * p.head_groups;
+  const int64_t steps = (keys + attn_step(pair) - 1) / attn_step(pair);
+  const int64_t workers = units * (steps <= p.snap ? 1 : steps);
+  *grid = static_cast<int>(std::min<int64_t>(*grid, pair ? workers : (workers + 1) / 2));
   return SVDMLP_OK;
 }
 
@@ -252,8 +269,13 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   common_params(&p, a, a->q_tokens);
   p.k_tokens = a->k_tokens;
   p.causal = a->causal != 0;
-  // one row tile holds the mean request: two workers instead of a second row tile that would mostly be empty
-  const bool pair = static_cast<int64_t>(a->q_tokens) * p.gp > 128ll * a->batch;
+  // Two row tiles that share their keys pay once the key walks are long; short
+  // requests gain more from two independent workers (measured, us, pair / solo:
+  // 16 heads of 64, 24 sequences of 140 tokens 30.8 / 25.1, 16 of 400 46 / 40, 8
+  // of 512 27.1 / 29.1; 32 and 8 heads of 128, 16 of 400 76 / 69, 8 of 512 54 / 54,
+  // 4 of 1024 80 / 90).  At most 128 rows leave the second tile empty.
+  const bool pair =
+      static_cast<int64_t>(a->q_tokens) * p.gp > 128ll * a->batch && a->k_tokens >= 512ll * a->batch;
   p.cu_k = a->cu_k;
   p.k = a->k;
   p.v = a->v;
@@ -261,14 +283,14 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   p.k_head = a->k_head;
   p.v_token = a->v_token;
   p.v_head = a->v_head;
+  const int step = attn_step(pair), box[3] = {64, 1, step};
+  p.snap = 512 / step;
   int grid = 0;
-  SVD_CHECK(attn_grid(&grid));
+  SVD_CHECK(attn_grid(p, pair, a->q_tokens, a->k_tokens, &grid));
   CUtensorMap mq, mk, mv;
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->q_tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[3] = {a->head_dim, a->kv_heads, a->k_tokens};
   const int64_t ks[3] = {1, a->k_head, a->k_token}, vs[3] = {1, a->v_head, a->v_token};
-  const int step = attn_step(pair), box[3] = {64, 1, step};
-  p.snap = 512 / step;
   SVD_CHECK(attn_map(&mk, a->dtype, a->k, 3, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v, 3, dims, vs, box));
   return pair ? dispatch_attention<false, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
@@ -306,15 +328,15 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   p.v = a->v_cache;
   p.k_token = a->k_block;
   p.v_token = a->v_block;
+  const int step = attn_step(pair), box[4] = {64, std::min(a->block_size, step), 1, 1};
+  p.snap = 512 / step;
   int grid = 0;
-  SVD_CHECK(attn_grid(&grid));
+  SVD_CHECK(attn_grid(p, pair, a->tokens, static_cast<int64_t>(a->table_width) * a->block_size, &grid));
   CUtensorMap mq, mk, mv;
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[4] = {a->head_dim, a->block_size, a->kv_heads, a->num_blocks};
   const int64_t head = static_cast<int64_t>(a->block_size) * a->head_dim;
   const int64_t ks[4] = {1, a->head_dim, head, a->k_block}, vs[4] = {1, a->head_dim, head, a->v_block};
-  const int step = attn_step(pair), box[4] = {64, std::min(a->block_size, step), 1, 1};
-  p.snap = 512 / step;
   SVD_CHECK(attn_map(&mk, a->dtype, a->k_cache, 4, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v_cache, 4, dims, vs, box));
   return pair ? dispatch_attention<true, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)

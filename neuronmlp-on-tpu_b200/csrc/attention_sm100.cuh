@@ -26,8 +26,8 @@
 // the unit's counter joins them in the order of the keys, so results do not
 // depend on the order of arrival.
 //
-// Roles (384 threads): two softmax warpgroups, one thread per row; MMA and TMA
-// warps.  TMEM (512 columns): per group two score tiles of 64 keys (the
+// Roles (384 threads): two softmax warpgroups, one thread per row; an MMA and a
+// TMA warp per worker.  TMEM (512 columns): per group two score tiles of 64 keys (the
 // probabilities overwrite them as 16-bit pairs and are the A operand of the
 // second product) and one output tile.  Scores run two steps ahead: the MMA
 // warp issues P V(j) and then Q K(j + 2), which takes P(j)'s place, while the
@@ -60,7 +60,6 @@ struct AttnParams {
   int snap;                           // units of up to this many steps are not divided
   float c;                            // |scale| log2(e)
   int neg;                            // scale < 0
-  int wide;                           // the output's rows lie on 32-byte boundaries
   const int *cu_q, *cu_k;             // packed keys
   const int *lens, *table;            // paged keys
   const long long* mask;
@@ -79,6 +78,11 @@ template <int D, bool PAIR>
 struct AttnCfg {
   static constexpr int HALVES = D / 64;
   static constexpr int WORKERS = PAIR ? 1 : 2;              // per CTA
+  // Registers of a softmax thread and of the other warps, when moved between
+  // them (three warps share a partition's 16 K: 168 each at launch).  PAIR holds
+  // 128 scores a thread; with 64 the softmax fits in 168, and the MMA and TMA
+  // warps run without spills (measured: 65 K decoding 66 -> 58 us).
+  static constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 104;
   static constexpr int Q_BYTES = 128 * D * 2;               // one row tile of q
   static constexpr int STEP = PAIR ? 128 : 64;              // keys per step
   static constexpr int SLOT_BYTES = STEP * D * 2;           // k or v of one step
@@ -189,19 +193,6 @@ template <int N>
 SVD_DEV void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 SVD_DEV void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// 32 bytes as one store (a whole sector), or two where the address is 16-byte aligned only.
-SVD_DEV void store_32(void* at, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
-                      uint32_t h, bool wide) {
-  if (wide) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(a), "r"(b), "r"(c), "r"(d),
-                 "r"(e), "r"(f), "r"(g), "r"(h)
-                 : "memory");
-  } else {
-    reinterpret_cast<uint4*>(at)[0] = make_uint4(a, b, c, d);
-    reinterpret_cast<uint4*>(at)[1] = make_uint4(e, f, g, h);
-  }
-}
 
 SVD_DEV float exp2_approx(float x) {
   float y;
@@ -446,7 +437,7 @@ struct AttnShared {
   int abort_flag, last[2];
   AttnCut cut[3];
   long long per;
-  long long scan[kAttnThreads / 32];
+  long long scan[12];
   long long rem[3];
   float m[256], l[256];         // joining: per-row maximum and 1 / sum
 };
@@ -455,6 +446,7 @@ struct AttnShared {
 constexpr uint32_t kInfoRow0 = 1, kInfoRow1 = 2;  // row tiles that the step counts for
 constexpr uint32_t kInfoFirst = 4, kInfoLast = 8; // first, last step of the segment
 constexpr uint32_t kInfoEnd = 16;                 // k: the worker's last step
+constexpr uint32_t kInfoTile = 32;                // always set
 constexpr int kInfoValid = 8;                     // v: keys that exist, 0 to 64 (8 bits)
 constexpr int kInfoBad = 16;                      // k: blocks of the step outside the cache (8 bits)
 
@@ -563,6 +555,169 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
   }
 }
 
+// Joins the partials of workers c0 .. c1 into the output rows of their unit, in
+// the order of the keys; all threads of the worker that arrived last.  Returns
+// how often the threads met, -1 when that wait ran out.  Not inlined: its
+// registers would weigh on the softmax loop.
+template <typename T, int D, bool PAIR>
+__device__ __noinline__ int attn_join(const AttnParams& p, AttnShared* sh, WaitCtx ctx, int wk, int gtid,
+                                      uint32_t parity, int rows0, int rows, int c0, int c1, int token0, int head0) {
+  using Cfg = AttnCfg<D, PAIR>;
+  constexpr int GT = PAIR ? 256 : 128;  // threads of a worker
+  const int lane = static_cast<int>(lane_id());
+  const auto partial = [&](int c) -> const float* {
+    return p.partials + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS;
+  };
+  float* jm = sh->m + wk * 128;
+  float* jl = sh->l + wk * 128;
+  // per row: the common maximum and 1 / sum
+  const float* stats = p.partials + Cfg::PART_ROWS * D;
+  const auto stat = [&](int c) { return stats + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS; };
+  constexpr int LANES = D / 4, PER = 32 / LANES;  // solo: a warp per row, two at head_dim 64
+  const bool few = !PAIR && rows <= GT / 32 * PER;
+  if (!few && (gtid < rows0 || (PAIR && gtid >= 128 && gtid - 128 < rows - rows0))) {  // a thread per row
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(stat(c) + gtid));
+    if (mm == -INFINITY) mm = 0.f;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c)
+      ll += exp2_approx(__ldcg(stat(c) + gtid) - mm) * __ldcg(stat(c) + Cfg::PART_ROWS + gtid);
+    jm[gtid] = mm;
+    jl[gtid] = ll == 0.f ? 0.f : 1.f / ll;
+  }
+  if (!few) {
+    mbar_arrive(&sh->xchg[wk]);
+    if (!warp_wait(&sh->xchg[wk], parity, ctx, SITE_ATTN_XCHG)) return -1;
+  }
+  if constexpr (PAIR) {
+    // a thread per row, 32 elements at a time
+    if (gtid < rows0 || (gtid >= 128 && gtid - 128 < rows - rows0)) {
+      const float mm = jm[gtid], iv = jl[gtid];
+    const int rr = gtid & 127, tk = token0 + (gtid >> 7) * p.tt + rr / p.gp, hd = head0 + rr % p.gp;
+    T* dst = static_cast<T*>(p.out) + static_cast<long long>(tk) * p.out_token + hd * p.out_head;
+#pragma unroll 1
+      for (int x = 0; x < D; x += 32) {
+        float acc[32];
+#pragma unroll
+        for (int y = 0; y < 32; ++y) acc[y] = 0.f;
+#pragma unroll 2
+        for (int c = c0; c <= c1; ++c) {
+          const float f = exp2_approx(__ldcg(stat(c) + gtid) - mm);
+          const float4* from = reinterpret_cast<const float4*>(partial(c)) + x / 4 * Cfg::PART_ROWS + gtid;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float4 o = __ldcg(from + y * Cfg::PART_ROWS);
+            acc[4 * y] = fmaf(f, o.x, acc[4 * y]);
+            acc[4 * y + 1] = fmaf(f, o.y, acc[4 * y + 1]);
+            acc[4 * y + 2] = fmaf(f, o.z, acc[4 * y + 2]);
+            acc[4 * y + 3] = fmaf(f, o.w, acc[4 * y + 3]);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < 32; y += 16) {
+          uint32_t o[8];
+#pragma unroll
+          for (int z = 0; z < 8; ++z) o[z] = pack_pair<T>(acc[y + 2 * z] * iv, acc[y + 2 * z + 1] * iv);
+          reinterpret_cast<uint4*>(dst + x + y)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          reinterpret_cast<uint4*>(dst + x + y)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+    }
+  } else {
+    const int sub = lane / LANES, d4 = lane % LANES;
+    const auto put = [&](int x, float4 a, float iv) {
+      const int tk = token0 + x / p.gp, hd = head0 + x % p.gp;
+      uint2 o;
+      o.x = pack_pair<T>(a.x * iv, a.y * iv);
+      o.y = pack_pair<T>(a.z * iv, a.w * iv);
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<long long>(tk) * p.out_token +
+                                hd * p.out_head + d4 * 4) = o;
+    };
+    if (few) {
+      // one row each: statistics and outputs of 16 partials in flight, joined as they come
+      constexpr int C = 16;
+      const int x = (gtid >> 5) * PER + sub;
+      if (x < rows) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll 1
+        for (int b0 = c0; b0 <= c1; b0 += C) {
+          float4 o[C];
+          float f[C], g[C];
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const int c = min(b0 + k, c1);
+            f[k] = __ldcg(stat(c) + x);
+            g[k] = __ldcg(stat(c) + Cfg::PART_ROWS + x);
+            o[k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
+          }
+          float top = mm;
+#pragma unroll
+          for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
+          const float safe = top == -INFINITY ? 0.f : top;
+          const float old = exp2_approx(mm - safe);
+          mm = top;
+          ll *= old;
+          acc.x *= old;
+          acc.y *= old;
+          acc.z *= old;
+          acc.w *= old;
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const float e = b0 + k <= c1 ? exp2_approx(f[k] - safe) : 0.f;
+            ll = fmaf(e, g[k], ll);
+            acc.x = fmaf(e, o[k].x, acc.x);
+            acc.y = fmaf(e, o[k].y, acc.y);
+            acc.z = fmaf(e, o[k].z, acc.z);
+            acc.w = fmaf(e, o[k].w, acc.w);
+          }
+        }
+        put(x, acc, ll == 0.f ? 0.f : 1.f / ll);
+      }
+    } else {
+      constexpr int U = 4, C = 4;             // rows and partials in flight
+      for (int x0 = (gtid >> 5) * PER + sub; x0 < rows; x0 += GT / 32 * PER * U) {
+        float4 acc[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int b0 = c0; b0 <= c1; b0 += C) {
+          float4 o[U][C];
+          float f[U][C];
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+            const int c = min(b0 + k, c1);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
+              o[u][k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
+              f[u][k] = __ldcg(stat(c) + x);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < C; ++k) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const float e = b0 + k <= c1 ? exp2_approx(f[u][k] - jm[min(x0 + u * (GT / 32 * PER), rows - 1)]) : 0.f;
+              acc[u].x = fmaf(e, o[u][k].x, acc[u].x);
+              acc[u].y = fmaf(e, o[u][k].y, acc[u].y);
+              acc[u].z = fmaf(e, o[u][k].z, acc[u].z);
+              acc[u].w = fmaf(e, o[u][k].w, acc[u].w);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int x = x0 + u * (GT / 32 * PER);
+          if (x < rows) put(x, acc[u], jl[x]);
+        }
+      }
+    }
+  }
+  return few ? 0 : 1;
+}
+
 template <typename T, int D, bool PAGED, bool PAIR>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -575,6 +730,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   static_assert(Cfg::OFF_BAR + sizeof(AttnShared) <= Cfg::SMEM_BYTES && Cfg::SMEM_BYTES <= 232448, "shared memory");
   static_assert(Cfg::WORKERS * Cfg::SLOTS <= 16, "barriers");
   if ((smem_addr(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
+    grid_dependency_wait();
     if (threadIdx.x == 0) atomicCAS(p.err, 0, SITE_ATTN_ALIGN);
     return;
   }
@@ -586,7 +742,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&sh->q_full[i], 1);
       mbar_init(&sh->q_empty[i], 1);
       for (int b = 0; b < 2; ++b) {
-        mbar_init(&sh->s_full[i][b], 2);  // the scores, and what is said of them
+        mbar_init(&sh->s_full[i][b], PAGED ? 2 : 1);  // the scores, and what is said of them
         mbar_init(&sh->p_ready[i][b], 128);
         mbar_init(&sh->pv_done[i][b], 1);
       }
@@ -608,6 +764,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     tmem_relinquish();
     tc_fence_before();
   }
+  grid_dependency_wait();
+  grid_launch_dependents();
   find_cuts<Cfg::WORKERS, PAIR>(p, sh);
   __syncthreads();
   tc_fence_after();
@@ -620,7 +778,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int STEP = Cfg::STEP, AHEAD = Cfg::TILES;  // the scores run AHEAD steps before the values
 
   if (warp >= 8) {
-    reg_dealloc<88>();
+    if constexpr (PAIR) reg_dealloc<Cfg::OTHER_REGS>();
     uint8_t* ring = smem + Cfg::OFF_KV + wk * Cfg::SLOTS * Cfg::SLOT_BYTES;
     uint64_t* kv_full = sh->kv_full + wk * Cfg::SLOTS;
     uint64_t* kv_empty = sh->kv_empty + wk * Cfg::SLOTS;
@@ -669,7 +827,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       };
       // row tiles that step j counts for, and whether it begins or ends the segment
       const auto about = [&](const Walk& at, int j, int st0, int st1) {
-        return (j < st0 ? kInfoRow0 : 0u) | (PAIR && j < st1 ? kInfoRow1 : 0u) | (j == at.j0 ? kInfoFirst : 0u) |
+        return kInfoTile | (j < st0 ? kInfoRow0 : 0u) | (PAIR && j < st1 ? kInfoRow1 : 0u) | (j == at.j0 ? kInfoFirst : 0u) |
                (j + 1 == at.j1 ? kInfoLast : 0u);
       };
       Walk wv = w;         // v follows k by AHEAD steps
@@ -750,38 +908,49 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
         return got;
       };
+      // Iteration g issues P V(g - AHEAD) and Q K(g).  Its waits for tiles, and
+      // the slots that it hands back, lie between the products of the one
+      // before: the tensor pipe has a few MMAs queued then, and goes idle when
+      // all of them come in one place (measured: 1150 cycles of each 3650).
       int stop = more ? INT_MAX : 0;           // known once the last k has come
-      for (int g = 0; g < stop; ++g) {
-        const bool do_v = g >= AHEAD, do_k = stop == INT_MAX;
-        uint32_t iv = 0, ik = 0;
-        int sv = 0, sk = 0;
-        if (do_v) {
-          sv = take(&iv);
-          const int valid = iv >> kInfoValid & 0xff;
-          if (ok && valid < STEP) {
-            // rows behind the last key are other requests' or nobody's: zeros
-            uint8_t* t = ring + sv * Cfg::SLOT_BYTES;
-            for (int x = valid * 8 + lane; x < STEP * 8; x += 32)
-              for (int hf = 0; hf < Cfg::HALVES; ++hf)
-                *reinterpret_cast<uint4*>(t + hf * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
+      uint32_t iv = 0, ik = 0;
+      int sv = 0, sk = 0;
+      const auto fetch_v = [&](int g) {
+        iv = 0;
+        if (g < AHEAD || g >= stop) return;
+        sv = take(&iv);
+        const int valid = iv >> kInfoValid & 0xff;
+        if (ok && valid < STEP) {
+          // rows behind the last key are other requests' or nobody's: zeros
+          uint8_t* t = ring + sv * Cfg::SLOT_BYTES;
+          for (int x = valid * 8 + lane; x < STEP * 8; x += 32)
+            for (int hf = 0; hf < Cfg::HALVES; ++hf)
+              *reinterpret_cast<uint4*>(t + hf * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
         }
-        if (do_k) {
-          sk = take(&ik);
-          if ((ik & kInfoEnd) != 0) stop = g + 1 + AHEAD;
-          if ((ik & kInfoFirst) != 0) {
-            ok = ok && warp_wait(&sh->q_full[wk], q_phase, ctx, SITE_ATTN_Q);
-            q_phase ^= 1;
-          }
+      };
+      const auto fetch_k = [&](int g) {
+        ik = 0;
+        if (stop != INT_MAX) return;
+        sk = take(&ik);
+        if ((ik & kInfoEnd) != 0) stop = g + 1 + AHEAD;
+        if ((ik & kInfoFirst) != 0) {
+          ok = ok && warp_wait(&sh->q_full[wk], q_phase, ctx, SITE_ATTN_Q);
+          q_phase ^= 1;
         }
+      };
+      if (more) fetch_k(0);
+      for (int g = 0; g < stop && ok; ++g) {
+        const bool do_v = g >= AHEAD, do_k = ik != 0;
+        const uint32_t jv = iv, jk = ik;
+        const int lv = sv, lk = sk;
 #pragma unroll
         for (int x = 0; x < GN; ++x) {
           const int i = wk + x;                // group
           const uint32_t mine = x == 0 ? kInfoRow0 : kInfoRow1;
           const uint32_t t_s = tmem + i * 128, t_o = tmem + 256 + i * D;
-          if ((iv & mine) != 0) {              // O (+)= P V, 64 keys at a time
+          if ((jv & mine) != 0) {              // O (+)= P V, 64 keys at a time
 #pragma unroll
             for (int hf = 0; hf < STEP / 64; ++hf) {
               // one barrier per 64 probabilities: the halves of a tile, or the two tiles in turn
@@ -789,29 +958,31 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               ok = ok && warp_wait(&sh->p_ready[i][b], PAIR ? n_p[x] & 1 : n_p[x] >> 1 & 1, ctx, SITE_ATTN_P);
               if (!ok) break;
               tc_fence_after();
-              umma_values(t_o, t_s + b * (PAIR ? 32 : 64), v_desc + (sv * Cfg::SLOT_BYTES + hf * 64 * 128) / 16, idesc_o,
-                          hf > 0 || (iv & kInfoFirst) == 0);
+              umma_values(t_o, t_s + b * (PAIR ? 32 : 64), v_desc + (lv * Cfg::SLOT_BYTES + hf * 64 * 128) / 16, idesc_o,
+                          hf > 0 || (jv & kInfoFirst) == 0);
             }
             if (ok) umma_commit_elected(&sh->pv_done[i][PAIR ? 0 : n_p[x] & 1]);
             ++n_p[x];
           }
-          if (ok && (ik & mine) != 0) {        // S = Q K^T
+          if (x == GN - 1 && do_v && ok) umma_commit_elected(&kv_empty[lv]);
+          if (ok && (jk & mine) != 0) {        // S = Q K^T
             const int b = PAIR ? 0 : n_q[x] & 1;
             tc_fence_after();
             umma_scores<D / 16, Cfg::HALF_BYTES>(t_s + b * 64, q_desc + x * (Cfg::Q_BYTES / 16),
-                                                 k_desc + sk * (Cfg::SLOT_BYTES / 16), idesc_s);
+                                                 k_desc + lk * (Cfg::SLOT_BYTES / 16), idesc_s);
             umma_commit_elected(&sh->s_full[i][b]);
-            if (lane == 0) {
-              sh->score_info[i][b] = ik;
+            if (PAGED && lane == 0) {
+              sh->score_info[i][b] = jk;
               mbar_arrive(&sh->s_full[i][b]);
             }
             ++n_q[x];
           }
+          if (x == 0 && ok) fetch_v(g + 1);
         }
         if (!ok) break;
-        if (do_v) umma_commit_elected(&kv_empty[sv]);
-        if (do_k) umma_commit_elected(&kv_empty[sk]);
-        if ((ik & kInfoLast) != 0) umma_commit_elected(&sh->q_empty[wk]);  // the last product with this q is issued
+        if (do_k) umma_commit_elected(&kv_empty[lk]);
+        if ((jk & kInfoLast) != 0) umma_commit_elected(&sh->q_empty[wk]);  // the last product with this q is issued
+        fetch_k(g + 1);
       }
       umma_commit_elected(&sh->drain[wk]);
       __syncwarp();
@@ -819,12 +990,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else {
     // -------------------------------------------------------- softmax groups
-    reg_alloc<208>();
+    if constexpr (PAIR) reg_alloc<Cfg::SOFTMAX_REGS>();
     const int i = warp >> 2;                          // group: row tile, S and O
     const int r = threadIdx.x & 127;                  // row of the tile, lane of TMEM
     const int ti = PAIR ? i : 0;                      // row tile of the unit
     const int gtid = PAIR ? threadIdx.x : r;          // thread of the worker
-    constexpr int GT = PAIR ? 256 : 128;              // threads of a worker
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + i * 128, t_o = tmem + lanes + 256 + i * D;
     const int row_token = r / p.gp, row_head = r - row_token * p.gp;
@@ -1001,7 +1171,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
                 for (int z = 0; z < 8; ++z)
                   o[z] = pack_pair<T>(__uint_as_float(v[y + 2 * z]) * inv, __uint_as_float(v[y + 2 * z + 1]) * inv);
-                store_32(dst + x + y, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], p.wide);
+                reinterpret_cast<uint4*>(dst + x + y)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                reinterpret_cast<uint4*>(dst + x + y)[1] = make_uint4(o[4], o[5], o[6], o[7]);
               }
             } else {
 #pragma unroll
@@ -1013,8 +1184,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                   __stcg(at + Cfg::PART_ROWS, make_float4(__uint_as_float(v[y + 4]), __uint_as_float(v[y + 5]),
                                                           __uint_as_float(v[y + 6]), __uint_as_float(v[y + 7])));
                 } else {               // [row][element]: few rows, a warp reads whole rows
-                  store_32(part + row * D + x + y, v[y], v[y + 1], v[y + 2], v[y + 3], v[y + 4], v[y + 5], v[y + 6],
-                           v[y + 7], true);
+                  __stcg(reinterpret_cast<uint4*>(part + row * D + x + y), make_uint4(v[y], v[y + 1], v[y + 2], v[y + 3]));
+                  __stcg(reinterpret_cast<uint4*>(part + row * D + x + y) + 1,
+                         make_uint4(v[y + 4], v[y + 5], v[y + 6], v[y + 7]));
                 }
               }
             }
@@ -1048,150 +1220,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       tc_fence_before();
       if (!whole) {
-        // the last worker of the unit to arrive joins the partials, in the order of the keys
+        // The last worker of the unit to arrive joins the partials, in the order of the keys.
+        __threadfence();
         if (!(ok = meet())) break;
         const long long unit0 = w.at - (w.j0 == 0 ? 0 : kUnitCost + w.j0);
         const int c0 = static_cast<int>(quotient(unit0 + kUnitCost, sh->per));
         const int c1 = static_cast<int>(quotient(unit0 + kUnitCost + w.steps - 1, sh->per));
         if (gtid == 0) {
-          __threadfence();
           const int arrived = atom_add_acq_rel_gpu(&p.counters[c0], 1);
           sh->last[wk] = arrived == c1 - c0;
           if (arrived == c1 - c0) p.counters[c0] = 0;
         }
         if (!(ok = meet())) break;
         if (sh->last[wk]) {
-          __threadfence();
-          const auto partial = [&](int c) -> const float* {
-            return p.partials + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS;
-          };
           const int rows0 = w.row_tokens(p, 0) * p.gp;
           const int rows = rows0 + (PAIR ? w.row_tokens(p, 1) * p.gp : 0);
-          float* jm = sh->m + wk * 128;
-          float* jl = sh->l + wk * 128;
-          // per row: the common maximum and 1 / sum
-          const float* stats = p.partials + Cfg::PART_ROWS * D;
-          const auto stat = [&](int c) { return stats + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS; };
-          if (!PAIR && rows <= 16) {                  // a warp per row, lanes over the partials
-            for (int x = gtid >> 5; x < rows; x += GT / 32) {
-              float mm = -INFINITY, ll = 0.f;
-              for (int b0 = c0; b0 <= c1; b0 += 32) {
-                const int c = b0 + lane;
-                const float mv = c <= c1 ? __ldcg(stat(c) + x) : -INFINITY;
-                const float lv = c <= c1 ? __ldcg(stat(c) + Cfg::PART_ROWS + x) : 0.f;
-                float top = fmaxf(mm, mv);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float safe = top == -INFINITY ? 0.f : top;
-                float sum = exp2_approx(mv - safe) * lv;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                ll = ll * exp2_approx(mm - safe) + sum;
-                mm = top;
-              }
-              if (lane == 0) {
-                jm[x] = mm == -INFINITY ? 0.f : mm;
-                jl[x] = ll == 0.f ? 0.f : 1.f / ll;
-              }
-            }
-          } else if (gtid < rows0 || (PAIR && gtid >= 128 && gtid - 128 < rows - rows0)) {  // a thread per row
-            float mm = -INFINITY, ll = 0.f;
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(stat(c) + gtid));
-            if (mm == -INFINITY) mm = 0.f;
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c)
-              ll += exp2_approx(__ldcg(stat(c) + gtid) - mm) * __ldcg(stat(c) + Cfg::PART_ROWS + gtid);
-            jm[gtid] = mm;
-            jl[gtid] = ll == 0.f ? 0.f : 1.f / ll;
-          }
-          if (!(ok = meet())) break;
-          if constexpr (PAIR) {
-            // a thread per row, 32 elements at a time
-            if (gtid < rows0 || (gtid >= 128 && gtid - 128 < rows - rows0)) {
-              const float mm = jm[gtid], iv = jl[gtid];
-#pragma unroll 1
-              for (int x = 0; x < D; x += 32) {
-                float acc[32];
-#pragma unroll
-                for (int y = 0; y < 32; ++y) acc[y] = 0.f;
-#pragma unroll 2
-                for (int c = c0; c <= c1; ++c) {
-                  const float f = exp2_approx(__ldcg(stat(c) + gtid) - mm);
-                  const float4* from = reinterpret_cast<const float4*>(partial(c)) + x / 4 * Cfg::PART_ROWS + gtid;
-#pragma unroll
-                  for (int y = 0; y < 8; ++y) {
-                    const float4 o = __ldcg(from + y * Cfg::PART_ROWS);
-                    acc[4 * y] = fmaf(f, o.x, acc[4 * y]);
-                    acc[4 * y + 1] = fmaf(f, o.y, acc[4 * y + 1]);
-                    acc[4 * y + 2] = fmaf(f, o.z, acc[4 * y + 2]);
-                    acc[4 * y + 3] = fmaf(f, o.w, acc[4 * y + 3]);
-                  }
-                }
-#pragma unroll
-                for (int y = 0; y < 32; y += 16) {
-                  uint32_t o[8];
-#pragma unroll
-                  for (int z = 0; z < 8; ++z) o[z] = pack_pair<T>(acc[y + 2 * z] * iv, acc[y + 2 * z + 1] * iv);
-                  store_32(dst + x + y, o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], p.wide);
-                }
-              }
-            }
-          } else {
-            // a warp per row (two at head_dim 64), U rows and C partials at a time
-            constexpr int LANES = D / 4, PER = 32 / LANES;
-            const int sub = lane / LANES, d4 = lane % LANES;
-            const auto join = [&](auto u_, auto c_) {
-              constexpr int U = decltype(u_)::value, C = decltype(c_)::value;
-              for (int x0 = (gtid >> 5) * PER + sub; x0 < rows; x0 += GT / 32 * PER * U) {
-                float4 acc[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int b0 = c0; b0 <= c1; b0 += C) {
-                  float4 o[U][C];
-                  float f[U][C];
-#pragma unroll
-                  for (int k = 0; k < C; ++k) {
-                    const int c = min(b0 + k, c1);
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                      const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
-                      o[u][k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
-                      f[u][k] = __ldcg(stat(c) + x);
-                    }
-                  }
-#pragma unroll
-                  for (int k = 0; k < C; ++k) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                      const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
-                      const float e = b0 + k <= c1 ? exp2_approx(f[u][k] - jm[x]) : 0.f;
-                      acc[u].x = fmaf(e, o[u][k].x, acc[u].x);
-                      acc[u].y = fmaf(e, o[u][k].y, acc[u].y);
-                      acc[u].z = fmaf(e, o[u][k].z, acc[u].z);
-                      acc[u].w = fmaf(e, o[u][k].w, acc[u].w);
-                    }
-                  }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                  const int x = x0 + u * (GT / 32 * PER);
-                  if (x < rows) {
-                    const float iv = jl[x];
-                    const int tk = w.t0(p, 0) + x / p.gp, hd = w.h * p.gp + x % p.gp;
-                    uint2 o;
-                    o.x = pack_pair<T>(acc[u].x * iv, acc[u].y * iv);
-                    o.y = pack_pair<T>(acc[u].z * iv, acc[u].w * iv);
-                    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<long long>(w.s.q0 + tk) * p.out_token +
-                                              hd * p.out_head + d4 * 4) = o;
-                  }
-                }
-              }
-            };
-            if (rows <= GT / 32 * PER) join(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-            else join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-          }
-          if (!(ok = meet())) break;  // jm and jl may be written again
+          const int met = attn_join<T, D, PAIR>(p, sh, ctx, wk, gtid, n_x & 1, rows0, rows, c0, c1, w.s.q0 + w.t0(p, 0),
+                                                w.h * p.gp);
+          ok = met >= 0;
+          if (!ok) break;
+          n_x += met;
         }
       }
     }

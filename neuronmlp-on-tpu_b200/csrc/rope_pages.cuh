@@ -53,6 +53,7 @@ template <typename T, int E>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
   extern __shared__ float2 turn[];  // [tile][half]
   using Vec = ElemVec<T, E>;
+  grid_dependency_wait();  // no early launch of the next kernel: its waiting CTAs would take this one's places
   const int t0 = blockIdx.x * p.tile;
   const int nt = min(p.tile, p.tokens - t0);
   for (int i = threadIdx.x; i < nt * p.half; i += kRopeThreads) {
@@ -182,6 +183,8 @@ __global__ void __launch_bounds__(kPagesThreads) page_step_kernel(const PagesPar
   __shared__ int s_take[kPagesChunk];      // blocks taken before it
   __shared__ int s_held[kPagesChunk];
   __shared__ unsigned long long s_warp[kPagesThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int left = max(0, min(*p.free_count, p.capacity));
   int cu0 = 0, take0 = 0;  // carried over the chunks
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -87,6 +87,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == device.index and t.is_contiguous():
+            return t
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError(f"{name} must be a {str(dtype)[6:]} tensor")
     if t.shape != shape:
@@ -97,6 +102,12 @@ def _index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device:
 
 
 def _offsets(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    try:
+        if (t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] > 1 and t.get_device() == device.index
+                and t.is_contiguous()):
+            return t
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
     if t.dim() != 1 or t.shape[0] < 2:
@@ -335,6 +346,29 @@ def kv_cache(num_blocks: int, kv_heads: int, block_size: int, head_dim: int, *, 
     return both[0], both[1]
 
 
+def _check_pages(block_table, seq_lens, new_lens, free_blocks, free_count, block_size, num_tokens):
+    """Raises what is wrong with page_step's arguments; the index tensors, contiguous."""
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.dim() != 2 or min(block_table.shape) <= 0 or block_table.stride(1) != 1:
+        raise ValueError(f"block_table must be a nonempty row-major [batch, width], got {tuple(block_table.shape)}")
+    if not block_table.is_cuda:
+        raise ValueError("block_table must be a CUDA tensor (the B200 path has no CPU fallback)")
+    device = block_table.device
+    b = block_table.shape[0]
+    seq_lens = _index("seq_lens", seq_lens, torch.int32, (b,), device)
+    new_lens = _index("new_lens", new_lens, torch.int32, (b,), device)
+    free_count = _index("free_count", free_count, torch.int32, (1,), device)
+    if not isinstance(free_blocks, torch.Tensor) or free_blocks.dtype != torch.int32:
+        raise TypeError("free_blocks must be an int32 tensor")
+    if free_blocks.dim() != 1 or not free_blocks.is_contiguous() or free_blocks.device != device:
+        raise ValueError("free_blocks must be a contiguous 1D tensor on the table's device")
+    ops._positive("block_size", block_size)
+    if isinstance(num_tokens, bool) or not isinstance(num_tokens, int) or num_tokens < 0:
+        raise ValueError(f"num_tokens must be a nonnegative integer, got {num_tokens}")
+    return seq_lens, new_lens, free_count
+
+
 def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks: torch.Tensor,
               free_count: torch.Tensor, block_size: int, num_tokens: int) -> PageStep:
     """Block tables, slots and positions of one forward pass from request lengths.
@@ -348,24 +382,24 @@ def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     free_count for the next step, and frees blocks by writing them behind
     free_count.  `missing` above zero means that the free list ran out: those
     blocks' entries and slots are -1."""
-    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
-        raise TypeError("block_table must be an int32 tensor")
-    if block_table.dim() != 2 or min(block_table.shape) <= 0 or block_table.stride(1) != 1:
-        raise ValueError(f"block_table must be a nonempty row-major [batch, width], got {tuple(block_table.shape)}")
-    if not block_table.is_cuda:
-        raise ValueError("block_table must be a CUDA tensor (the B200 path has no CPU fallback)")
+    try:
+        b, width = block_table.shape
+        index, one = block_table.get_device(), (1,)
+        want = seq_lens.shape
+        good = (index >= 0 and width > 0 and b > 0 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
+                and want == (b,) and seq_lens.dtype is torch.int32 and seq_lens.get_device() == index
+                and new_lens.shape == want and new_lens.dtype is torch.int32 and new_lens.get_device() == index
+                and free_count.shape == one and free_count.dtype is torch.int32 and free_count.get_device() == index
+                and free_blocks.dtype is torch.int32 and free_blocks.get_device() == index and free_blocks.dim() == 1
+                and seq_lens.is_contiguous() and new_lens.is_contiguous() and free_blocks.is_contiguous()
+                and type(block_size) is int and block_size > 0 and type(num_tokens) is int and num_tokens >= 0)
+    except (AttributeError, TypeError, ValueError):
+        good = False
+    if not good:
+        seq_lens, new_lens, free_count = _check_pages(block_table, seq_lens, new_lens, free_blocks, free_count, block_size,
+                                                      num_tokens)
+        b, width = block_table.shape
     device = block_table.device
-    b, width = block_table.shape
-    seq_lens = _index("seq_lens", seq_lens, torch.int32, (b,), device)
-    new_lens = _index("new_lens", new_lens, torch.int32, (b,), device)
-    free_count = _index("free_count", free_count, torch.int32, (1,), device)
-    if not isinstance(free_blocks, torch.Tensor) or free_blocks.dtype != torch.int32:
-        raise TypeError("free_blocks must be an int32 tensor")
-    if free_blocks.dim() != 1 or not free_blocks.is_contiguous() or free_blocks.device != device:
-        raise ValueError("free_blocks must be a contiguous 1D tensor on the table's device")
-    ops._positive("block_size", block_size)
-    if isinstance(num_tokens, bool) or not isinstance(num_tokens, int) or num_tokens < 0:
-        raise ValueError(f"num_tokens must be a nonnegative integer, got {num_tokens}")
     slots = torch.empty(num_tokens, dtype=torch.int64, device=device)
     whole = torch.empty(num_tokens + 2 * b + 3, dtype=torch.int32, device=device)
     at = whole.data_ptr()
