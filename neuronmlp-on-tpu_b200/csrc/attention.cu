@@ -48,9 +48,11 @@ static int launch_overlapped(void (*kernel)(Params...), int grid, int threads, s
 
 // --------------------------------------------------------------------- rope
 template <typename T, int E>
-static int launch_rope(const RopeParams& p, cudaStream_t s) {
-  return launch_overlapped(rope_kernel<T, E>, (p.tokens + p.tile - 1) / p.tile, kRopeThreads,
-                           static_cast<size_t>(p.tile) * p.half * sizeof(float2), s, p);
+static int launch_rope(const RopeParams& p, bool interleaved, cudaStream_t s) {
+  const int grid = (p.tokens + p.tile - 1) / p.tile;
+  const size_t smem = static_cast<size_t>(p.tile) * p.half * sizeof(float2);
+  return interleaved ? launch_overlapped(rope_kernel<T, E, true>, grid, kRopeThreads, smem, s, p)
+                     : launch_overlapped(rope_kernel<T, E, false>, grid, kRopeThreads, smem, s, p);
 }
 
 static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
@@ -74,11 +76,7 @@ static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
   p.kv_heads = a->kv_heads;
   p.head_dim = a->head_dim;
   p.half = a->rotary_dim / 2;
-  p.interleaved = a->interleaved != 0;
   p.block_size = a->block_size;
-  p.block_shift = -1;
-  if (cached && (a->block_size & (a->block_size - 1)) == 0)
-    for (p.block_shift = 0; (1 << p.block_shift) < a->block_size;) ++p.block_shift;
   p.scale = a->scale;
   p.q = a->q;
   p.k = a->k;
@@ -99,7 +97,6 @@ static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
   p.k_block = a->k_block;
   p.v_block = a->v_block;
   p.cache_slots = static_cast<long long>(a->block_size) * a->num_blocks;
-  p.tile = std::max(1, std::min(kRopeMaxTile, a->tokens / (4 * planning_sms())));
   bool vec = p.half % 8 == 0 && p.head_dim % 8 == 0 && rows_aligned(p.q, p.q_token, p.q_head) &&
              rows_aligned(p.k, p.k_token, p.k_head) && rows_aligned(p.q_out, 0, 0) && rows_aligned(p.k_out, 0, 0);
   if (cached)
@@ -108,9 +105,16 @@ static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
   if (!elems_aligned(p.q) || !elems_aligned(p.k) || !elems_aligned(p.v) || !elems_aligned(p.q_out) ||
       !elems_aligned(p.k_out) || !elems_aligned(p.k_cache) || !elems_aligned(p.v_cache))
     return SVDMLP_ERR_ALIGNMENT;
+  const int e = vec ? 8 : 1;
+  p.rot_units = p.half / e;
+  p.head_units = p.rot_units + (p.head_dim - 2 * p.half) / e;
+  p.v_units = p.head_dim / e;
+  // fewer tokens per CTA where the tokens would not fill the SMs several times over
+  p.tile = std::max(1, std::min(kRopeTile, a->tokens / (4 * planning_sms())));
+  const bool inter = a->interleaved != 0;
   if (a->dtype == SVDMLP_BF16)
-    return vec ? launch_rope<__nv_bfloat16, 8>(p, s) : launch_rope<__nv_bfloat16, 1>(p, s);
-  return vec ? launch_rope<__half, 8>(p, s) : launch_rope<__half, 1>(p, s);
+    return vec ? launch_rope<__nv_bfloat16, 8>(p, inter, s) : launch_rope<__nv_bfloat16, 1>(p, inter, s);
+  return vec ? launch_rope<__half, 8>(p, inter, s) : launch_rope<__half, 1>(p, inter, s);
 }
 
 // -------------------------------------------------------------------- pages

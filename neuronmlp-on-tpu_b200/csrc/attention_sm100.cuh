@@ -221,16 +221,6 @@ SVD_DEV float2 add2(float2 a, float2 b) {
   return d;
 }
 
-template <typename T>
-SVD_DEV uint32_t pack_pair(float lo, float hi);
-template <>
-SVD_DEV uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-template <>
-SVD_DEV uint32_t pack_pair<__half>(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
 // --------------------------------------------------------------- the cutting
 SVD_DEV long long quotient(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);

@@ -43,6 +43,7 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 # checks have to as well); only where that fails, _refuse_* name what is wrong.
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch.cuda.current_device
+_PLAIN = torch.contiguous_format
 
 
 def _refuse_dtype(t) -> None:
@@ -139,11 +140,12 @@ def _check_caches(k_cache, v_cache, like: torch.Tensor, kv_heads: Optional[int])
     """(num_blocks, kv_heads, block_size, stride between k blocks, between v blocks), or an exception."""
     try:
         nb, hk, bs, d = shape = k_cache.shape
-        kb, *inner = k_cache.stride()
-        vb, *inner_v = v_cache.stride()
-        if (inner == inner_v == [bs * d, d, 1] and v_cache.shape == shape and nb * hk * bs > 0
+        kb, k1, k2, k3 = k_cache.stride()
+        vb, v1, v2, v3 = v_cache.stride()
+        if (k3 == v3 == 1 and k2 == v2 == d and k1 == v1 == bs * d and v_cache.shape == shape and nb * hk * bs > 0
                 and d == like.shape[2] and (kv_heads is None or hk == kv_heads)
-                and k_cache.dtype is v_cache.dtype is like.dtype and k_cache.device == v_cache.device == like.device):
+                and k_cache.dtype is v_cache.dtype is like.dtype
+                and k_cache.get_device() == v_cache.get_device() == like.get_device()):
             return nb, hk, bs, kb, vb
     except (AttributeError, TypeError, ValueError):
         pass
@@ -269,12 +271,19 @@ def _rope(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, sc
     if nk != n:
         raise ValueError("q and k must have the same tokens: dimensions do not match")
     positions = _index("positions", positions, torch.int32, (n,), device)
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype is not torch.float32:
-        raise TypeError("inv_freq must be a float32 tensor")
-    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must be [rotary_dim / 2] with rotary_dim at most {d}, got {tuple(inv_freq.shape)}")
-    if inv_freq.device != device:
-        raise ValueError("inputs must be CUDA tensors on one device")
+    try:
+        half, = inv_freq.shape
+        good = (inv_freq.dtype is torch.float32 and 0 < 2 * half <= d and inv_freq.get_device() == device.index
+                and inv_freq.is_contiguous())
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype is not torch.float32:
+            raise TypeError("inv_freq must be a float32 tensor")
+        if inv_freq.device != device:
+            raise ValueError("inputs must be CUDA tensors on one device")
+        raise ValueError(f"inv_freq must be a contiguous [rotary_dim / 2] with rotary_dim at most {d}, "
+                         f"got {tuple(inv_freq.shape)}")
     q_token, q_head, unit = q.stride()
     if unit != 1:
         q = q.contiguous()
@@ -294,11 +303,11 @@ def _rope(q, k, v, positions, slots, inv_freq, k_cache, v_cache, interleaved, sc
             v = v.contiguous()
             v_token, v_head, unit = v.stride()
         v_ptr, slots_ptr, kc, vc = v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    q_out = torch.empty((n, h, d), dtype=dtype, device=device)
-    k_out = torch.empty((n, hk, d), dtype=dtype, device=device) if return_k else None
+    q_out = torch.empty_like(q, memory_format=_PLAIN)
+    k_out = torch.empty_like(k, memory_format=_PLAIN) if return_k else None
     if n == 0:
         return q_out, k_out
-    args = _lib.ROPE_ARGS(code, n, h, hk, d, 2 * inv_freq.shape[0], 1 if interleaved else 0, bs, nb, scale,
+    args = _lib.ROPE_ARGS(code, n, h, hk, d, 2 * half, 1 if interleaved else 0, bs, nb, scale,
                           q.data_ptr(), k.data_ptr(), v_ptr, q_token, q_head, k_token, k_head, v_token, v_head,
                           positions.data_ptr(), slots_ptr, inv_freq.data_ptr(), q_out.data_ptr(),
                           k_out.data_ptr() if return_k else 0, kc, vc, kb, vb)
@@ -459,7 +468,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if cu_k.shape != cu_q.shape:
             raise ValueError("cu_q and cu_k must have matching shapes")
     scale = _scale(scale, d)
-    out = torch.empty((nq, h, d), dtype=dtype, device=device) if out is None else _output(out, q)
+    out = torch.empty_like(q, memory_format=_PLAIN) if out is None else _output(out, q)
     if nq == 0:
         return out
     if nk == 0:
@@ -524,7 +533,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         mask_ptr = tree_mask.data_ptr()
     ops._positive("max_tree", max_tree)
     scale = _scale(scale, d)
-    out = torch.empty((n, h, d), dtype=dtype, device=device) if out is None else _output(out, q)
+    out = torch.empty_like(q, memory_format=_PLAIN) if out is None else _output(out, q)
     if n == 0:
         return out
     q = _rows(q)
