@@ -30,9 +30,9 @@ static bool elems_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p
 // kernels waits on the device (griddepcontrol.wait) before it reads or writes
 // anything, and lets its own successor launch at once.
 template <typename... Params, typename... Args>
-static int launch_overlapped(void (*kernel)(Params...), int grid, int threads, size_t smem, cudaStream_t s, Args&&... args) {
+static int launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args&&... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -51,8 +51,8 @@ template <typename T, int E>
 static int launch_rope(const RopeParams& p, bool interleaved, cudaStream_t s) {
   const int grid = (p.tokens + p.tile - 1) / p.tile;
   const size_t smem = static_cast<size_t>(p.tile) * p.half * sizeof(float2);
-  return interleaved ? launch_overlapped(rope_kernel<T, E, true>, grid, kRopeThreads, smem, s, p)
-                     : launch_overlapped(rope_kernel<T, E, false>, grid, kRopeThreads, smem, s, p);
+  return interleaved ? launch_overlapped(rope_kernel<T, E, true>, dim3(grid), kRopeThreads, smem, s, p)
+                     : launch_overlapped(rope_kernel<T, E, false>, dim3(grid), kRopeThreads, smem, s, p);
 }
 
 static int rope_impl(const svdmlp_rope_args* a, cudaStream_t s) {
@@ -145,7 +145,7 @@ static int pages_impl(const svdmlp_pages_args* a, cudaStream_t s) {
   p.count_out = a->count_out;
   p.missing = a->missing;
   const int grid = std::max(1, std::min(planning_sms(), (a->tokens + kPagesThreads - 1) / kPagesThreads));
-  return launch_overlapped(page_step_kernel, grid, kPagesThreads, 0, s, p);
+  return launch_overlapped(page_step_kernel, dim3(grid), kPagesThreads, 0, s, p);
 }
 
 // ---------------------------------------------------------------- attention
@@ -188,16 +188,17 @@ static int query_map(CUtensorMap* map, int dtype, const void* q, int tokens, int
 
 // ------------------------------------------------------------------- launch
 static constexpr int64_t kAttnCtlBytes = 256, kAttnCounterBytes = 1 << 20;  // as svdmlp_workspace_init lays them out
+static constexpr int64_t kAttnSplitBytes = 2 * kAttnMaxGrid * sizeof(AttnSplit);
 
 template <int D>
 static int64_t attn_workspace() {
-  return kAttnCtlBytes + kAttnCounterBytes +
+  return kAttnCtlBytes + kAttnCounterBytes + kAttnSplitBytes +
          static_cast<int64_t>(std::min(planning_sms(), kAttnMaxGrid)) * 2 * AttnCfg<D, true>::PART_FLOATS * 4;
 }
 
 template <typename T, int D, bool PAGED, bool PAIR>
 static int launch_attention(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnParams& p,
-                            int grid, cudaStream_t s) {
+                            int grid, int join_rows, cudaStream_t s) {
   constexpr int SMEM = AttnCfg<D, PAIR>::SMEM_BYTES;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
   int dev = 0;
@@ -206,18 +207,24 @@ static int launch_attention(const CUtensorMap& q, const CUtensorMap& k, const CU
     SVD_CUDA(cudaFuncSetAttribute(attention_kernel<T, D, PAGED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  return launch_overlapped(attention_kernel<T, D, PAGED, PAIR>, grid, kAttnThreads, SMEM, s, q, k, v, p);
+  SVD_CHECK(launch_overlapped(attention_kernel<T, D, PAGED, PAIR>, dim3(grid), kAttnThreads, SMEM, s, q, k, v, p));
+  if (join_rows == 0) return SVDMLP_OK;
+  constexpr int PER = PAIR ? 32 : kJoinThreads / 32 * (128 / D);
+  return launch_overlapped(attention_join_kernel<T, D, PAIR>, dim3(grid * AttnCfg<D, PAIR>::WORKERS, (join_rows + PER - 1) / PER),
+                           kJoinThreads, 0, s, p);
 }
 
 template <bool PAGED, bool PAIR>
 static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                              const AttnParams& p, int grid, cudaStream_t s) {
+                              const AttnParams& p, int grid, int join_rows, cudaStream_t s) {
   if (dtype == SVDMLP_BF16)
-    return head_dim == 128 ? launch_attention<__nv_bfloat16, 128, PAGED, PAIR>(q, k, v, p, grid, s)
-                           : launch_attention<__nv_bfloat16, 64, PAGED, PAIR>(q, k, v, p, grid, s);
-  return head_dim == 128 ? launch_attention<__half, 128, PAGED, PAIR>(q, k, v, p, grid, s)
-                         : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, s);
+    return head_dim == 128 ? launch_attention<__nv_bfloat16, 128, PAGED, PAIR>(q, k, v, p, grid, join_rows, s)
+                           : launch_attention<__nv_bfloat16, 64, PAGED, PAIR>(q, k, v, p, grid, join_rows, s);
+  return head_dim == 128 ? launch_attention<__half, 128, PAGED, PAIR>(q, k, v, p, grid, join_rows, s)
+                         : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, join_rows, s);
 }
+
+static constexpr int kPromptSnap = 1024, kTreePairSnap = 512, kTreeSnap = 512;
 
 // Keys per step.
 static int attn_step(bool pair) { return pair ? AttnCfg<128, true>::STEP : AttnCfg<128, false>::STEP; }
@@ -243,20 +250,23 @@ static void common_params(AttnParams* p, const Args* a, int q_tokens) {
   p->out_head = a->out_head;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p->err = reinterpret_cast<int*>(ws);
-  p->counters = reinterpret_cast<int*>(ws + kAttnCtlBytes);
-  p->partials = reinterpret_cast<float*>(ws + kAttnCtlBytes + kAttnCounterBytes);
+  p->splits = reinterpret_cast<AttnSplit*>(ws + kAttnCtlBytes + kAttnCounterBytes);
+  p->partials = reinterpret_cast<float*>(ws + kAttnCtlBytes + kAttnCounterBytes + kAttnSplitBytes);
   p->timeout_ns = wait_limit_ns();
 }
 
 // One CTA per SM, or fewer where there cannot be work for all: at most `tokens`
-// rows in `batch` requests, of at most `keys` keys each.
-static int attn_grid(const AttnParams& p, bool pair, int64_t tokens, int64_t keys, int* grid) {
+// rows in `batch` requests, of at most `keys` keys each.  join_rows: rows of a
+// unit that the join has to expect, 0 where no unit can be divided.
+static int attn_grid(const AttnParams& p, bool pair, int64_t tokens, int64_t keys, int64_t unit_rows, int* grid,
+                     int* join_rows) {
   SVD_CHECK(device_sms(grid));
   *grid = std::min(*grid, kAttnMaxGrid);
   const int64_t units = (tokens / (pair ? 2 * p.tt : p.tt) + p.batch) * p.head_groups;
   const int64_t steps = (keys + attn_step(pair) - 1) / attn_step(pair);
   const int64_t workers = units * (steps <= p.snap ? 1 : steps);
   *grid = static_cast<int>(std::min<int64_t>(*grid, pair ? workers : (workers + 1) / 2));
+  *join_rows = steps <= p.snap ? 0 : static_cast<int>(std::min<int64_t>(unit_rows, pair ? 256 : 128));
   return SVDMLP_OK;
 }
 
@@ -288,17 +298,17 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   p.v_token = a->v_token;
   p.v_head = a->v_head;
   const int step = attn_step(pair), box[3] = {64, 1, step};
-  p.snap = 512 / step;
-  int grid = 0;
-  SVD_CHECK(attn_grid(p, pair, a->q_tokens, a->k_tokens, &grid));
+  p.snap = kPromptSnap / step;
+  int grid = 0, join_rows = 0;
+  SVD_CHECK(attn_grid(p, pair, a->q_tokens, a->k_tokens, static_cast<int64_t>(a->q_tokens) * p.gp, &grid, &join_rows));
   CUtensorMap mq, mk, mv;
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->q_tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[3] = {a->head_dim, a->kv_heads, a->k_tokens};
   const int64_t ks[3] = {1, a->k_head, a->k_token}, vs[3] = {1, a->v_head, a->v_token};
   SVD_CHECK(attn_map(&mk, a->dtype, a->k, 3, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v, 3, dims, vs, box));
-  return pair ? dispatch_attention<false, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
-              : dispatch_attention<false, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
+  return pair ? dispatch_attention<false, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, join_rows, s)
+              : dispatch_attention<false, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, join_rows, s);
 }
 
 static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
@@ -333,9 +343,10 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   p.k_token = a->k_block;
   p.v_token = a->v_block;
   const int step = attn_step(pair), box[4] = {64, std::min(a->block_size, step), 1, 1};
-  p.snap = 512 / step;
-  int grid = 0;
-  SVD_CHECK(attn_grid(p, pair, a->tokens, static_cast<int64_t>(a->table_width) * a->block_size, &grid));
+  p.snap = (pair ? kTreePairSnap : kTreeSnap) / step;
+  int grid = 0, join_rows = 0;
+  SVD_CHECK(attn_grid(p, pair, a->tokens, static_cast<int64_t>(a->table_width) * a->block_size,
+                      pair ? 256 : static_cast<int64_t>(a->max_tree) * p.gp, &grid, &join_rows));
   CUtensorMap mq, mk, mv;
   SVD_CHECK(query_map(&mq, a->dtype, a->q, a->tokens, a->q_heads, a->head_dim, p.gp, a->q_token, a->q_head));
   const int64_t dims[4] = {a->head_dim, a->block_size, a->kv_heads, a->num_blocks};
@@ -343,8 +354,8 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   const int64_t ks[4] = {1, a->head_dim, head, a->k_block}, vs[4] = {1, a->head_dim, head, a->v_block};
   SVD_CHECK(attn_map(&mk, a->dtype, a->k_cache, 4, dims, ks, box));
   SVD_CHECK(attn_map(&mv, a->dtype, a->v_cache, 4, dims, vs, box));
-  return pair ? dispatch_attention<true, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s)
-              : dispatch_attention<true, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, s);
+  return pair ? dispatch_attention<true, true>(a->dtype, a->head_dim, mq, mk, mv, p, grid, join_rows, s)
+              : dispatch_attention<true, false>(a->dtype, a->head_dim, mq, mk, mv, p, grid, join_rows, s);
 }
 
 }  // namespace svdmlp

@@ -22,9 +22,11 @@
 // the request lengths on the device, so ragged lengths, long prompts and a
 // single long context load every SM alike.  A cut inside a short unit moves to
 // the unit's start.  A unit that a cut divides leaves fp32 partials (maximum,
-// sum, unnormalised output) in the workspace; the worker that arrives last at
-// the unit's counter joins them in the order of the keys, so results do not
-// depend on the order of arrival.
+// sum, unnormalised output) in the workspace, and the worker that begins it a
+// note of where they are; a second kernel joins them, in the order of the keys.
+// (Joined by the worker that arrives last instead, a CTA read up to a megabyte
+// on its own: 16 drafted tokens on 8000 keys 56 us, JOIN_A; 2 K decoding of 8
+// requests 27 us, JOIN_B.)
 //
 // Roles (384 threads): two softmax warpgroups, one thread per row; an MMA and a
 // TMA warp per worker.  TMEM (512 columns): per group two score tiles of 64 keys (the
@@ -50,8 +52,18 @@
 namespace svdmlp {
 
 constexpr int kAttnThreads = 384;
-constexpr int kAttnMaxGrid = 512;     // counters and partial slots reserved
+constexpr int kAttnMaxGrid = 512;     // CTAs that the workspace has room for
 constexpr float kAttnLazy = 8.0f;     // growth of the maximum (log2) that a stale base absorbs
+
+// What a worker leaves for the join: the unit that it begins and does not
+// finish.  Its partials are this worker's second one and the first ones of the
+// `more` workers after it.
+struct AttnSplit {
+  int more;             // 0: none
+  int rows0, rows;      // rows of the first row tile, of the unit
+  int token0, head0;    // first query row (in the tensor) and head
+  int pad[3];
+};
 
 struct AttnParams {
   int batch, q_tokens, k_tokens;
@@ -69,8 +81,9 @@ struct AttnParams {
   long long q_token, q_head, k_token, k_head, v_token, v_head;  // k_token, v_token: strides between blocks when paged
   void* out;
   long long out_token, out_head;
-  int *err, *counters;
+  int* err;
   float* partials;
+  struct AttnSplit* splits;           // per worker
   unsigned long long timeout_ns;
 };
 
@@ -98,7 +111,7 @@ struct AttnCfg {
 
 enum AttnSite : int {
   SITE_ATTN_Q = 31, SITE_ATTN_Q_EMPTY, SITE_ATTN_KV_FULL, SITE_ATTN_KV_EMPTY, SITE_ATTN_S, SITE_ATTN_P, SITE_ATTN_PV,
-  SITE_ATTN_XCHG, SITE_ATTN_DRAIN, SITE_ATTN_ALIGN
+  SITE_ATTN_DRAIN, SITE_ATTN_ALIGN
 };
 
 // ------------------------------------------------------------ tcgen05 forms
@@ -418,18 +431,17 @@ __device__ __noinline__ void attn_row(const AttnParams& p, const AttnSeq& s, int
 
 // -------------------------------------------------------------- the kernel
 struct AttnShared {
-  uint64_t q_full[2], q_empty[2], xchg[2], drain[2];
+  uint64_t q_full[2], q_empty[2], drain[2];
   uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];  // per group and score tile
   uint64_t kv_full[16], kv_empty[16];
   uint32_t slot_info[16];                // what the TMA warp says of a slot's tile
   uint32_t score_info[2][2];             // ... and the MMA warp hands on with the scores
   uint32_t tmem;
-  int abort_flag, last[2];
+  int abort_flag;
   AttnCut cut[3];
   long long per;
   long long scan[12];
   long long rem[3];
-  float m[256], l[256];         // joining: per-row maximum and 1 / sum
 };
 
 // Bits of a slot's info word.
@@ -545,167 +557,122 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
   }
 }
 
-// Joins the partials of workers c0 .. c1 into the output rows of their unit, in
-// the order of the keys; all threads of the worker that arrived last.  Returns
-// how often the threads met, -1 when that wait ran out.  Not inlined: its
-// registers would weigh on the softmax loop.
+// Joins the partials of divided units: block column c for the unit that worker c
+// begins (most begin none), block rows over its rows.  Statistics and outputs of
+// several partials are in flight at a time and joined as they come, with a
+// running maximum, in the order of the keys.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int D, bool PAIR>
-__device__ __noinline__ int attn_join(const AttnParams& p, AttnShared* sh, WaitCtx ctx, int wk, int gtid,
-                                      uint32_t parity, int rows0, int rows, int c0, int c1, int token0, int head0) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
   using Cfg = AttnCfg<D, PAIR>;
-  constexpr int GT = PAIR ? 256 : 128;  // threads of a worker
-  const int lane = static_cast<int>(lane_id());
+  grid_dependency_wait();
+  const int c0 = blockIdx.x;
+  const AttnSplit u = p.splits[c0];
+  if (u.more <= 0) return;
+  const int warp = threadIdx.x >> 5, lane = static_cast<int>(lane_id());
   const auto partial = [&](int c) -> const float* {
-    return p.partials + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS;
+    return p.partials + (2LL * (c0 + c) + (c == 0 ? 1 : 0)) * Cfg::PART_FLOATS;
   };
-  float* jm = sh->m + wk * 128;
-  float* jl = sh->l + wk * 128;
-  // per row: the common maximum and 1 / sum
-  const float* stats = p.partials + Cfg::PART_ROWS * D;
-  const auto stat = [&](int c) { return stats + (2LL * c + (c == c0 ? 1 : 0)) * Cfg::PART_FLOATS; };
-  constexpr int LANES = D / 4, PER = 32 / LANES;  // solo: a warp per row, two at head_dim 64
-  const bool few = !PAIR && rows <= GT / 32 * PER;
-  if (!few && (gtid < rows0 || (PAIR && gtid >= 128 && gtid - 128 < rows - rows0))) {  // a thread per row
-    float mm = -INFINITY, ll = 0.f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(stat(c) + gtid));
-    if (mm == -INFINITY) mm = 0.f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c)
-      ll += exp2_approx(__ldcg(stat(c) + gtid) - mm) * __ldcg(stat(c) + Cfg::PART_ROWS + gtid);
-    jm[gtid] = mm;
-    jl[gtid] = ll == 0.f ? 0.f : 1.f / ll;
-  }
-  if (!few) {
-    mbar_arrive(&sh->xchg[wk]);
-    if (!warp_wait(&sh->xchg[wk], parity, ctx, SITE_ATTN_XCHG)) return -1;
-  }
+  const auto row_at = [&](int row) -> T* {  // the output row
+    const int r = row & 127;
+    return static_cast<T*>(p.out) + static_cast<long long>(u.token0 + (row >> 7) * p.tt + r / p.gp) * p.out_token +
+           (u.head0 + r % p.gp) * p.out_head;
+  };
   if constexpr (PAIR) {
-    // a thread per row, 32 elements at a time
-    if (gtid < rows0 || (gtid >= 128 && gtid - 128 < rows - rows0)) {
-      const float mm = jm[gtid], iv = jl[gtid];
-    const int rr = gtid & 127, tk = token0 + (gtid >> 7) * p.tt + rr / p.gp, hd = head0 + rr % p.gp;
-    T* dst = static_cast<T*>(p.out) + static_cast<long long>(tk) * p.out_token + hd * p.out_head;
+    // partials [element / 4][row][4]: a lane per row, D / 8 elements per warp
+    constexpr int N = D / 32, C = 4;
+    for (int row = blockIdx.y * 32 + lane; row < 256; row += gridDim.y * 32) {
+      if (row < 128 ? row >= u.rows0 : row - 128 >= u.rows - u.rows0) continue;
+      float4 acc[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      float mm = -INFINITY, ll = 0.f;
 #pragma unroll 1
-      for (int x = 0; x < D; x += 32) {
-        float acc[32];
+      for (int b0 = 0; b0 <= u.more; b0 += C) {
+        float f[C], g[C];
+        float4 o[C][N];
 #pragma unroll
-        for (int y = 0; y < 32; ++y) acc[y] = 0.f;
-#pragma unroll 2
-        for (int c = c0; c <= c1; ++c) {
-          const float f = exp2_approx(__ldcg(stat(c) + gtid) - mm);
-          const float4* from = reinterpret_cast<const float4*>(partial(c)) + x / 4 * Cfg::PART_ROWS + gtid;
+        for (int k = 0; k < C; ++k) {
+          const float* from = partial(min(b0 + k, u.more));
+          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
+          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const float4 o = __ldcg(from + y * Cfg::PART_ROWS);
-            acc[4 * y] = fmaf(f, o.x, acc[4 * y]);
-            acc[4 * y + 1] = fmaf(f, o.y, acc[4 * y + 1]);
-            acc[4 * y + 2] = fmaf(f, o.z, acc[4 * y + 2]);
-            acc[4 * y + 3] = fmaf(f, o.w, acc[4 * y + 3]);
+          for (int n = 0; n < N; ++n)
+            o[k][n] = __ldcg(reinterpret_cast<const float4*>(from) + (warp * N + n) * Cfg::PART_ROWS + row);
+        }
+        float top = mm;
+#pragma unroll
+        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
+        const float safe = top == -INFINITY ? 0.f : top;
+        const float old = exp2_approx(mm - safe);
+        mm = top;
+        ll *= old;
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] = make_float4(acc[n].x * old, acc[n].y * old, acc[n].z * old, acc[n].w * old);
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+          const float e = b0 + k <= u.more ? exp2_approx(f[k] - safe) : 0.f;
+          ll = fmaf(e, g[k], ll);
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            acc[n].x = fmaf(e, o[k][n].x, acc[n].x);
+            acc[n].y = fmaf(e, o[k][n].y, acc[n].y);
+            acc[n].z = fmaf(e, o[k][n].z, acc[n].z);
+            acc[n].w = fmaf(e, o[k][n].w, acc[n].w);
           }
         }
-#pragma unroll
-        for (int y = 0; y < 32; y += 16) {
-          uint32_t o[8];
-#pragma unroll
-          for (int z = 0; z < 8; ++z) o[z] = pack_pair<T>(acc[y + 2 * z] * iv, acc[y + 2 * z + 1] * iv);
-          reinterpret_cast<uint4*>(dst + x + y)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          reinterpret_cast<uint4*>(dst + x + y)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        }
       }
+      const float iv = ll == 0.f ? 0.f : 1.f / ll;
+      uint4* to = reinterpret_cast<uint4*>(row_at(row) + warp * N * 4);
+#pragma unroll
+      for (int n = 0; n < N; n += 2)
+        to[n / 2] = make_uint4(pack_pair<T>(acc[n].x * iv, acc[n].y * iv), pack_pair<T>(acc[n].z * iv, acc[n].w * iv),
+                               pack_pair<T>(acc[n + 1].x * iv, acc[n + 1].y * iv),
+                               pack_pair<T>(acc[n + 1].z * iv, acc[n + 1].w * iv));
     }
   } else {
+    // partials [row][element]: a warp per row, two at head_dim 64
+    constexpr int LANES = D / 4, PER = 32 / LANES, C = 16;
     const int sub = lane / LANES, d4 = lane % LANES;
-    const auto put = [&](int x, float4 a, float iv) {
-      const int tk = token0 + x / p.gp, hd = head0 + x % p.gp;
-      uint2 o;
-      o.x = pack_pair<T>(a.x * iv, a.y * iv);
-      o.y = pack_pair<T>(a.z * iv, a.w * iv);
-      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<long long>(tk) * p.out_token +
-                                hd * p.out_head + d4 * 4) = o;
-    };
-    if (few) {
-      // one row each: statistics and outputs of 16 partials in flight, joined as they come
-      constexpr int C = 16;
-      const int x = (gtid >> 5) * PER + sub;
-      if (x < rows) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float mm = -INFINITY, ll = 0.f;
+    constexpr int ROWS = kJoinThreads / 32 * PER;
+    for (int row = (blockIdx.y * (kJoinThreads / 32) + warp) * PER + sub; row < u.rows; row += gridDim.y * ROWS) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float mm = -INFINITY, ll = 0.f;
 #pragma unroll 1
-        for (int b0 = c0; b0 <= c1; b0 += C) {
-          float4 o[C];
-          float f[C], g[C];
+      for (int b0 = 0; b0 <= u.more; b0 += C) {
+        float4 o[C];
+        float f[C], g[C];
 #pragma unroll
-          for (int k = 0; k < C; ++k) {
-            const int c = min(b0 + k, c1);
-            f[k] = __ldcg(stat(c) + x);
-            g[k] = __ldcg(stat(c) + Cfg::PART_ROWS + x);
-            o[k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
-          }
-          float top = mm;
-#pragma unroll
-          for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
-          const float safe = top == -INFINITY ? 0.f : top;
-          const float old = exp2_approx(mm - safe);
-          mm = top;
-          ll *= old;
-          acc.x *= old;
-          acc.y *= old;
-          acc.z *= old;
-          acc.w *= old;
-#pragma unroll
-          for (int k = 0; k < C; ++k) {
-            const float e = b0 + k <= c1 ? exp2_approx(f[k] - safe) : 0.f;
-            ll = fmaf(e, g[k], ll);
-            acc.x = fmaf(e, o[k].x, acc.x);
-            acc.y = fmaf(e, o[k].y, acc.y);
-            acc.z = fmaf(e, o[k].z, acc.z);
-            acc.w = fmaf(e, o[k].w, acc.w);
-          }
+        for (int k = 0; k < C; ++k) {
+          const float* from = partial(min(b0 + k, u.more));
+          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
+          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
+          o[k] = __ldcg(reinterpret_cast<const float4*>(from + row * D) + d4);
         }
-        put(x, acc, ll == 0.f ? 0.f : 1.f / ll);
-      }
-    } else {
-      constexpr int U = 4, C = 4;             // rows and partials in flight
-      for (int x0 = (gtid >> 5) * PER + sub; x0 < rows; x0 += GT / 32 * PER * U) {
-        float4 acc[U];
+        float top = mm;
 #pragma unroll
-        for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (int b0 = c0; b0 <= c1; b0 += C) {
-          float4 o[U][C];
-          float f[U][C];
+        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);
+        const float safe = top == -INFINITY ? 0.f : top;
+        const float old = exp2_approx(mm - safe);
+        mm = top;
+        ll *= old;
+        acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
 #pragma unroll
-          for (int k = 0; k < C; ++k) {
-            const int c = min(b0 + k, c1);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int x = min(x0 + u * (GT / 32 * PER), rows - 1);
-              o[u][k] = __ldcg(reinterpret_cast<const float4*>(partial(c) + x * D) + d4);
-              f[u][k] = __ldcg(stat(c) + x);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < C; ++k) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const float e = b0 + k <= c1 ? exp2_approx(f[u][k] - jm[min(x0 + u * (GT / 32 * PER), rows - 1)]) : 0.f;
-              acc[u].x = fmaf(e, o[u][k].x, acc[u].x);
-              acc[u].y = fmaf(e, o[u][k].y, acc[u].y);
-              acc[u].z = fmaf(e, o[u][k].z, acc[u].z);
-              acc[u].w = fmaf(e, o[u][k].w, acc[u].w);
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int x = x0 + u * (GT / 32 * PER);
-          if (x < rows) put(x, acc[u], jl[x]);
+        for (int k = 0; k < C; ++k) {
+          const float e = b0 + k <= u.more ? exp2_approx(f[k] - safe) : 0.f;
+          ll = fmaf(e, g[k], ll);
+          acc.x = fmaf(e, o[k].x, acc.x);
+          acc.y = fmaf(e, o[k].y, acc.y);
+          acc.z = fmaf(e, o[k].z, acc.z);
+          acc.w = fmaf(e, o[k].w, acc.w);
         }
       }
+      const float iv = ll == 0.f ? 0.f : 1.f / ll;
+      *reinterpret_cast<uint2*>(row_at(row) + d4 * 4) =
+          make_uint2(pack_pair<T>(acc.x * iv, acc.y * iv), pack_pair<T>(acc.z * iv, acc.w * iv));
     }
   }
-  return few ? 0 : 1;
 }
 
 template <typename T, int D, bool PAGED, bool PAIR>
@@ -736,7 +703,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         mbar_init(&sh->p_ready[i][b], 128);
         mbar_init(&sh->pv_done[i][b], 1);
       }
-      mbar_init(&sh->xchg[i], PAIR ? 256 : 128);
       mbar_init(&sh->drain[i], 1);
     }
     for (int i = 0; i < Cfg::WORKERS * Cfg::SLOTS; ++i) {
@@ -984,18 +950,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int i = warp >> 2;                          // group: row tile, S and O
     const int r = threadIdx.x & 127;                  // row of the tile, lane of TMEM
     const int ti = PAIR ? i : 0;                      // row tile of the unit
-    const int gtid = PAIR ? threadIdx.x : r;          // thread of the worker
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + i * 128, t_o = tmem + lanes + 256 + i * D;
     const int row_token = r / p.gp, row_head = r - row_token * p.gp;
-    unsigned n_s = 0, n_x = 0;                        // score tiles taken; exchanges
+    unsigned n_s = 0;                                 // score tiles taken
     bool ok = true;
-    const auto meet = [&]() {                         // all threads of the worker
-      mbar_arrive(&sh->xchg[wk]);
-      const bool k = warp_wait(&sh->xchg[wk], n_x & 1, ctx, SITE_ATTN_XCHG);
-      ++n_x;
-      return k;
-    };
+    AttnSplit split{};
     for (; more; more = w.next(p)) {
       const int steps_i = w.row_steps(p, ti);
       const int t0 = w.t0(p, ti), token = t0 + row_token;
@@ -1209,30 +1169,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
       }
       tc_fence_before();
-      if (!whole) {
-        // The last worker of the unit to arrive joins the partials, in the order of the keys.
-        __threadfence();
-        if (!(ok = meet())) break;
-        const long long unit0 = w.at - (w.j0 == 0 ? 0 : kUnitCost + w.j0);
-        const int c0 = static_cast<int>(quotient(unit0 + kUnitCost, sh->per));
-        const int c1 = static_cast<int>(quotient(unit0 + kUnitCost + w.steps - 1, sh->per));
-        if (gtid == 0) {
-          const int arrived = atom_add_acq_rel_gpu(&p.counters[c0], 1);
-          sh->last[wk] = arrived == c1 - c0;
-          if (arrived == c1 - c0) p.counters[c0] = 0;
-        }
-        if (!(ok = meet())) break;
-        if (sh->last[wk]) {
-          const int rows0 = w.row_tokens(p, 0) * p.gp;
-          const int rows = rows0 + (PAIR ? w.row_tokens(p, 1) * p.gp : 0);
-          const int met = attn_join<T, D, PAIR>(p, sh, ctx, wk, gtid, n_x & 1, rows0, rows, c0, c1, w.s.q0 + w.t0(p, 0),
-                                                w.h * p.gp);
-          ok = met >= 0;
-          if (!ok) break;
-          n_x += met;
-        }
+      if (!whole && w.j0 == 0) {                      // the worker's last segment: others go on with the unit
+        const long long unit = w.at + kUnitCost;
+        split.more = static_cast<int>(quotient(unit + w.steps - 1, sh->per) - quotient(unit, sh->per));
+        split.rows0 = w.row_tokens(p, 0) * p.gp;
+        split.rows = split.rows0 + (PAIR ? w.row_tokens(p, 1) * p.gp : 0);
+        split.token0 = w.s.q0 + w.t0(p, 0);
+        split.head0 = w.h * p.gp;
       }
     }
+    if (r == 0 && ti == 0) p.splits[blockIdx.x * Cfg::WORKERS + wk] = ok ? split : AttnSplit{};
   }
 
   // rows of no request give zeros
