@@ -224,7 +224,7 @@ static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, con
                          : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, join_rows, s);
 }
 
-static constexpr int kPromptSnap = 1024, kTreePairSnap = 512, kTreeSnap = 512;
+static constexpr int kPromptSnap = 1024, kTreeSnap = 256;
 
 // Keys per step.
 static int attn_step(bool pair) { return pair ? AttnCfg<128, true>::STEP : AttnCfg<128, false>::STEP; }
@@ -343,7 +343,7 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   p.k_token = a->k_block;
   p.v_token = a->v_block;
   const int step = attn_step(pair), box[4] = {64, std::min(a->block_size, step), 1, 1};
-  p.snap = (pair ? kTreePairSnap : kTreeSnap) / step;
+  p.snap = kTreeSnap / step;
   int grid = 0, join_rows = 0;
   SVD_CHECK(attn_grid(p, pair, a->tokens, static_cast<int64_t>(a->table_width) * a->block_size,
                       pair ? 256 : static_cast<int64_t>(a->max_tree) * p.gp, &grid, &join_rows));

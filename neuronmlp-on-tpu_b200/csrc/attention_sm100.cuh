@@ -321,8 +321,11 @@ SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int w, int
 // On the line a unit is kUnitCost and its steps long: beginning and ending a
 // unit (q, the output) costs about as much as so many steps, and the early
 // tiles of a causal prompt are many units of few steps (measured: without it
-// the CTAs that got those finished 100 us after the others at 8192 tokens).
-constexpr int kUnitCost = 2;
+// the CTAs that got those finished 100 us after the others at 8192 tokens; 1, 2
+// and 4 for pairs: chunks behind 5600 keys 86, 75, 70 us; for the others
+// 64-request decoding 91, 84, 87 us).
+template <bool PAIR>
+constexpr int kUnitCost = PAIR ? 4 : 2;
 
 // A place on the line, and the unit and step it lies in.
 struct AttnCut {
@@ -354,12 +357,12 @@ struct AttnWalk {
   }
   SVD_DEV bool open(const AttnParams& p) {
     steps = tile_steps<STEP>(p, s, tokens(p), tile);
-    const long long left = end - at - (j0 == 0 ? kUnitCost : 0);
+    const long long left = end - at - (j0 == 0 ? kUnitCost<PAIR> : 0);
     j1 = left < steps - j0 ? j0 + static_cast<int>(left) : steps;
     return true;
   }
   SVD_DEV bool next(const AttnParams& p) {
-    at += j1 - j0 + (j0 == 0 ? kUnitCost : 0);
+    at += j1 - j0 + (j0 == 0 ? kUnitCost<PAIR> : 0);
     if (at >= end) return false;
     j0 = 0;
     if (++tile == tiles) {
@@ -481,7 +484,7 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
         s = load_seq(p, b);
         if (s.n > 0) {
           const int tiles = tiles_of(s, w);
-          const long long cost = steps_before<STEP>(p, s, w, tiles) + static_cast<long long>(tiles) * kUnitCost;
+          const long long cost = steps_before<STEP>(p, s, w, tiles) + static_cast<long long>(tiles) * kUnitCost<PAIR>;
           unit = static_cast<unsigned>(cost);
           mine = cost * p.head_groups;
         }
@@ -533,20 +536,20 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
     const AttnSeq s = sh->cut[k].s;
     int lo = 0, hi = tiles_of(s, w);  // lo is at or before it, hi beyond
     if (!p.causal) {
-      lo = static_cast<int>(quotient(rem, max(1, steps_of<STEP>(s.m)) + kUnitCost));
+      lo = static_cast<int>(quotient(rem, max(1, steps_of<STEP>(s.m)) + kUnitCost<PAIR>));
     } else {
       while (hi - lo > 1) {
         const int stride = (hi - lo + 31) / 32;
         const int x = lo + lane * stride;
-        const bool below = x < hi && steps_before<STEP>(p, s, w, x) + static_cast<long long>(x) * kUnitCost <= rem;
+        const bool below = x < hi && steps_before<STEP>(p, s, w, x) + static_cast<long long>(x) * kUnitCost<PAIR> <= rem;
         const int n = __popc(__ballot_sync(0xffffffffu, below));  // lane 0 always
         hi = min(hi, lo + n * stride);
         lo += (n - 1) * stride;
       }
     }
     if (lane == 0) {
-      const int in = static_cast<int>(rem - steps_before<STEP>(p, s, w, lo) - static_cast<long long>(lo) * kUnitCost);
-      int j = in - kUnitCost;
+      const int in = static_cast<int>(rem - steps_before<STEP>(p, s, w, lo) - static_cast<long long>(lo) * kUnitCost<PAIR>);
+      int j = in - kUnitCost<PAIR>;
       if (j <= 0 || tile_steps<STEP>(p, s, w, lo) <= p.snap) {  // at the unit's start
         sh->cut[k].at = at - in;
         j = 0;
@@ -1170,7 +1173,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       tc_fence_before();
       if (!whole && w.j0 == 0) {                      // the worker's last segment: others go on with the unit
-        const long long unit = w.at + kUnitCost;
+        const long long unit = w.at + kUnitCost<PAIR>;
         split.more = static_cast<int>(quotient(unit + w.steps - 1, sh->per) - quotient(unit, sh->per));
         split.rows0 = w.row_tokens(p, 0) * p.gp;
         split.rows = split.rows0 + (PAIR ? w.row_tokens(p, 1) * p.gp : 0);
