@@ -590,7 +590,7 @@ int svdmlp_rope(const svdmlp_rope_args* args, void* stream);
  * 0), cu[0 .. batch] their offsets, lens[b] = held + added, *count_out what is
  * left of the free list, *missing the blocks that it lacked (their entries and
  * slots are -1).  Only new table entries are written: the call may be
- * repeated.  Negative lengths count as 0. */
+ * repeated.  Negative lengths count as 0.  No output overlaps an input. */
 typedef struct svdmlp_pages_args {
   int32_t batch, tokens, block_size, table_width, free_capacity, reserved;
   int32_t* table; /* [batch, ld_table] */
@@ -606,7 +606,8 @@ int svdmlp_page_step(const svdmlp_pages_args* args, void* stream);
  * query i of n sees the first m - n + i + 1 of m keys (the queries are the last
  * n tokens).  out = softmax(scale q k^T) v; a row that sees no key gives zeros.
  * head_dim is 64 or 128; rows and heads 16-byte aligned.  `workspace`: at least
- * svdmlp_prompt_workspace_bytes, initialised by svdmlp_workspace_init. */
+ * svdmlp_prompt_workspace_bytes, initialised by svdmlp_workspace_init.  `out`
+ * overlaps no input, here and below. */
 typedef struct svdmlp_prompt_args {
   int32_t dtype, batch, q_tokens, k_tokens, q_heads, kv_heads, head_dim, causal;
   float scale;

@@ -224,6 +224,10 @@ static int dispatch_attention(int dtype, int head_dim, const CUtensorMap& q, con
                          : launch_attention<__half, 64, PAGED, PAIR>(q, k, v, p, grid, join_rows, s);
 }
 
+// Units of up to so many keys are not divided: partials and the join cost more
+// than the uneven end (measured, us).  Prompts, 512 / 1024 keys: 8 requests of
+// 100 to 600 tokens 35.7 / 29.6, 16 of 400 47.9 / 38.  Trees, 512 / 256: 64
+// requests of one token on some 800 keys 88 / 84, 8 on 2000 26 / 21.
 static constexpr int kPromptSnap = 1024, kTreeSnap = 256;
 
 // Keys per step.

@@ -6,15 +6,15 @@
 // the group for tt = 128 / gp tokens, row = token * gp + head (a group of more
 // than 64 heads is taken head by head).  Packing the group lets one tile of k
 // and v serve every head that shares it, fills the 128 rows of the MMA when
-// there are few tokens, and narrows the causal diagonal to tt tokens.  Keys are
-// walked in steps of 64.
+// there are few tokens, and narrows the causal diagonal to tt tokens.
 //
 // Two schedules (PAIR, chosen by the host).  A unit is one (request, head
 // group, token tile).  PAIR: a unit has two row tiles, which share every k and
-// v tile; for requests of more than 128 rows.  Otherwise a unit has one row
-// tile, and the CTA holds two independent workers, each with its own ring, MMA
-// warp and TMA warp, so that one's loads and epilogues lie beside the other's
-// products: a second row tile would be empty, and the bytes of k and v bound.
+// v tile, 128 keys per step; for requests of more than 128 rows.  Otherwise a
+// unit has one row tile, 64 keys per step, and the CTA holds two independent
+// workers, each with its own ring, MMA warp and TMA warp, so that one's loads
+// and epilogues lie beside the other's products: a second row tile would be
+// empty, and the bytes of k and v bound.
 //
 // Work.  The steps of all units, and a few steps' worth for every unit's
 // beginning and end, form one line, cut into equal pieces, one per
@@ -25,23 +25,31 @@
 // sum, unnormalised output) in the workspace, and the worker that begins it a
 // note of where they are; a second kernel joins them, in the order of the keys.
 // (Joined by the worker that arrives last instead, a CTA read up to a megabyte
-// on its own: 16 drafted tokens on 8000 keys 56 us, JOIN_A; 2 K decoding of 8
-// requests 27 us, JOIN_B.)
+// on its own: one request of 16 drafted tokens on 8000 keys 52 us, 25 us with
+// the second kernel; 8 requests of one token on 2000 keys 31 and 21 us.)
 //
 // Roles (384 threads): two softmax warpgroups, one thread per row; an MMA and a
-// TMA warp per worker.  TMEM (512 columns): per group two score tiles of 64 keys (the
-// probabilities overwrite them as 16-bit pairs and are the A operand of the
-// second product) and one output tile.  Scores run two steps ahead: the MMA
-// warp issues P V(j) and then Q K(j + 2), which takes P(j)'s place, while the
-// group already works on the scores of step j + 1, across the ends of units
-// too.  The output is rescaled only when a row's maximum grows by more than 8
-// (in powers of two): a stale base keeps probabilities below 2^8, which the
-// 16-bit types and the fp32 sums hold without loss.
+// TMA warp per worker.  TMEM (512 columns): per group 128 columns of scores and
+// one output tile.  The probabilities overwrite the scores as 16-bit pairs and
+// are the A operand of the second product.  With 64-key steps the 128 columns
+// are two score tiles, and the scores run two steps ahead: the MMA warp issues
+// P V(j) and then Q K(j + 2), which takes P(j)'s place, while the group already
+// works on the scores of step j + 1, across the ends of units too.  PAIR has one
+// tile of 128 keys per group, one step ahead, and the two groups take turns on
+// the tensor pipe and on the exponential unit; P V starts on the first 64 keys
+// while the exponentials of the others are computed.  (With two tiles of 64 the
+// MMA warp's waits and commits bound PAIR: 687 us where this takes 520, at one
+// prompt of 8192 tokens, 64 and 8 heads of 128.)  The output is rescaled only
+// when a row's maximum grows by more than 8 (in powers of two): a stale base
+// keeps probabilities below 2^8, which the 16-bit types and the fp32 sums hold
+// without loss.
 //
-// What bounds it: 64 keys x 128 rows cost 640 cycles of the tensor pipe at
-// head_dim 128 (its shared-memory reads: q and k for 64 columns take 48 cycles
-// per 16 elements where the products take 32) and 512 of the exponential unit;
-// with few rows the bytes of k and v.
+// What bounds it.  Long prompts: per 128 keys and 128 rows at head_dim 128 the
+// tensor pipe takes 1100 cycles and the exponential unit 1024, and the chain
+// scores -> maximum -> exponentials -> P V of the two tiles in turn leaves gaps
+// in both (42 and 47 % of the active cycles at 4096 tokens).  Few rows on many
+// keys: the bytes of k and v, read once; for short calls the start of the CTAs
+// (cuts, tensor maps, first loads: 2.5 us) and the join.
 #pragma once
 
 #include <climits>
@@ -83,7 +91,7 @@ struct AttnParams {
   long long out_token, out_head;
   int* err;
   float* partials;
-  struct AttnSplit* splits;           // per worker
+  AttnSplit* splits;           // per worker
   unsigned long long timeout_ns;
 };
 
@@ -478,15 +486,14 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
     for (int b0 = 0; b0 < p.batch; b0 += 128) {
       const int b = b0 + tid;
       long long mine = 0;
-      unsigned unit = 0;
+      long long unit = 0;
       AttnSeq s{};
       if (b < p.batch) {
         s = load_seq(p, b);
         if (s.n > 0) {
           const int tiles = tiles_of(s, w);
-          const long long cost = steps_before<STEP>(p, s, w, tiles) + static_cast<long long>(tiles) * kUnitCost<PAIR>;
-          unit = static_cast<unsigned>(cost);
-          mine = cost * p.head_groups;
+          unit = steps_before<STEP>(p, s, w, tiles) + static_cast<long long>(tiles) * kUnitCost<PAIR>;
+          mine = unit * p.head_groups;
         }
       }
       long long inc = mine;
@@ -692,6 +699,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if ((smem_addr(smem) & 1023u) != 0) {  // the swizzle counts from 1024-byte boundaries
     grid_dependency_wait();
     if (threadIdx.x == 0) atomicCAS(p.err, 0, SITE_ATTN_ALIGN);
+    if (threadIdx.x < Cfg::WORKERS) p.splits[blockIdx.x * Cfg::WORKERS + threadIdx.x] = AttnSplit{};  // nothing to join
     return;
   }
   const int warp = threadIdx.x >> 5;

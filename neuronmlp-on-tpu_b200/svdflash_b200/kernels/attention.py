@@ -168,6 +168,8 @@ def _output(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
         raise TypeError("out must have the inputs' dtype")
     if not _vector_rows(out, out.stride()):
         raise ValueError("out must have 16-byte aligned rows")
+    if out.data_ptr() == q.data_ptr() and q.numel():
+        raise ValueError("out must not overlap the inputs")
     return out
 
 

@@ -575,7 +575,8 @@ def test_python_refusals(cuda_device, att):
             (lambda: prompt(cu_q=cu.long()), TypeError), (lambda: prompt(cu_q=cu[:1]), ValueError),
             (lambda: prompt(cu_k=ref.cumulative([3, 3], cuda_device)), ValueError), (lambda: prompt(cu_q=cu.cpu()), ValueError),
             (lambda: prompt(scale=float("nan")), ValueError), (lambda: prompt(out=torch.empty_like(k)), ValueError),
-            (lambda: prompt(out=torch.empty_like(q).half()), TypeError),
+            (lambda: prompt(out=torch.empty_like(q).half()), TypeError), (lambda: prompt(out=q), ValueError),
+            (lambda: tree(out=q), ValueError),
             (lambda: tree(kc=kc[:, :, :12], vc=vc[:, :, :12]), ValueError), (lambda: tree(kc=kc.half()), TypeError),
             (lambda: tree(vc=vc[:3]), ValueError), (lambda: tree(max_tree=0), ValueError), (lambda: tree(max_tree=1.5), ValueError),
             (lambda: tree(lens=lens.long()), TypeError), (lambda: tree(table=table[0]), ValueError),
