@@ -52,7 +52,8 @@
 // same products take 395 instead of 490 us); in calls that follow one another
 // for long the power limit takes the clock down, to 540 us.  Few rows on many
 // keys: the bytes of k and v, read once; for short calls the start of the CTAs
-// (cuts, tensor maps, first loads: 2.5 us) and the join.
+// (the cuts 2 to 4 us, block tables and first loads 3) and the join.  One token on
+// 65537 keys: 54 us, 5.1 TB/s, and 5 us for the join.
 #pragma once
 
 #include <climits>
@@ -591,7 +592,8 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
 // Joins the partials of divided units: block column c for the unit that worker c
 // begins (most begin none), block rows over its rows.  Statistics and outputs of
 // several partials are in flight at a time and joined as they come, with a
-// running maximum, in the order of the keys.
+// running maximum, in the order of the keys.  Latency-bound: 5 us for 8 units of
+// 37 partials (8 key/value heads, one token on 65537 keys).
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D, bool PAIR>

@@ -229,7 +229,8 @@ constexpr int kPagesChunk = 1024;  // requests scanned at a time
 // finding its request by bisection; CTA 0 writes what there is one of per
 // request.  A token in a new block takes the block's number from the free list
 // itself, so no CTA waits for another's table entries.  Latency-bound: one
-// scan and one bisection stand between the loads and the stores.
+// scan and one bisection stand between the loads and the stores; 2.5 us for 8
+// requests of one token, 4.0 us for 1024 with up to 300 each (in a CUDA graph).
 __global__ void __launch_bounds__(kPagesThreads) page_step_kernel(const PagesParams p) {
   constexpr int PER = kPagesChunk / kPagesThreads;
   __shared__ int s_cu[kPagesChunk + 1];    // first new token of each request of the chunk
