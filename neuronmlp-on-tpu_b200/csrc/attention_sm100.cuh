@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const volatile uint32_t* slot_info = sh->slot_info + wk * Cfg::SLOTS;
       uint32_t phase = 0, q_phase = 0, turn = i == 0 ? 1 : 0;
       unsigned n_q = 0, n_p = 0;               // score and probability tiles so far
-      bool ok = true;
+      bool ok = true, had = false;             // had: P V in this segment (PAIR)
       // waits for the next slot of the ring, in the order of the loads
       const auto take = [&](uint32_t* info) -> int {
         ok = ok && warp_wait(&kv_full[slot], phase, ctx, SITE_ATTN_KV_FULL);
@@ -958,8 +958,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (!ok) break;
           if (!PAIR) umma_commit_elected(&sh->pv_done[i][n_p & 1]);
           ++n_p;
+          had = true;
         }
-        if (PAIR && (iv & kInfoLast) != 0) umma_commit_elected(&sh->pv_done[i][0]);
+        if (PAIR && (iv & kInfoLast) != 0) {
+          // only for a segment with steps for this tile: their probabilities hold
+          // the barrier's next phase back until every row has seen this one
+          if (had) umma_commit_elected(&sh->pv_done[i][0]);
+          had = false;
+        }
         if ((ik & kInfoFirst) != 0) {          // q comes late: the other tile's P V before it
           pass_turn();
           take_turn();
@@ -996,7 +1002,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + i * 128, t_o = tmem + lanes + 256 + i * D;
     const int row_token = r / p.gp, row_head = r - row_token * p.gp;
-    unsigned n_s = 0, n_seg = 0;                      // score tiles taken, segments ended
+    unsigned n_s = 0, n_seg = 0;                      // score tiles taken, segments with any
     bool ok = true;
     AttnSplit split{};
     for (; more; more = w.next(p)) {
@@ -1130,7 +1136,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok && *ctx.abort_flag == 0);
       if (!ok) break;
-      if (PAIR || some) {
+      if (PAIR ? last_j > w.j0 : some) {
         const unsigned last = n_s - 1;
         if (!(ok = warp_wait(&sh->pv_done[i][PAIR ? 0 : last & 1], PAIR ? n_seg & 1 : last >> 1 & 1, ctx, SITE_ATTN_PV))) break;
         tc_fence_after();

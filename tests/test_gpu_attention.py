@@ -549,6 +549,22 @@ def test_steps_through_the_cache_match_one_prompt(cuda_device, att):
         ref.check(torch.cat(outs[i]), want, mag, tiny, BF16, f"request {i}")
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lq,lk,h,hk,d,dtype", [
+    ([127, 50, 1949], [127, 0, 1949], 12, 4, 128, F16),                          # no keys between two long walks
+    ([60, 1, 40, 7, 900], [0, 0, 0, 0, 5000], 8, 2, 64, BF16),
+    ([300] + [2] * 40 + [500], [900] + [600] * 40 + [500], 4, 1, 128, BF16),     # second row tiles of nobody, one after another
+])
+def test_prompt_units_without_rows_or_keys(cuda_device, att, lq, lk, h, hk, d, dtype, causal):
+    """Units that have nothing for one or both row tiles, between units that have; the same every time."""
+    q, k, v = _qkv(sum(lk) + d, sum(lq), sum(lk), h, hk, d, dtype)
+    cq, ck = ref.cumulative(lq, cuda_device), ref.cumulative(lk, cuda_device)
+    outs = [att.prompt_attention(q, k, v, cq, ck, causal=causal) for _ in range(8)]
+    _status(cuda_device)
+    ref.check(outs[0], *ref.prompt(q, k, v, lq, lk, causal), dtype, f"{lq} {lk}")
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 # ----------------------------------------------------------------- refusals
 def test_python_refusals(cuda_device, att):
     q, k = _randn(1, 6, 4, 128), _randn(2, 6, 2, 128)
