@@ -287,13 +287,15 @@ static int prompt_impl(const svdmlp_prompt_args* a, cudaStream_t s) {
   common_params(&p, a, a->q_tokens);
   p.k_tokens = a->k_tokens;
   p.causal = a->causal != 0;
-  // Two row tiles that share their keys pay once the key walks are long; short
+  // Two row tiles that share their keys pay once the key walks are long; shorter
   // requests gain more from two independent workers (measured, us, pair / solo:
-  // 16 heads of 64, 24 sequences of 140 tokens 30.8 / 25.1, 16 of 400 46 / 40, 8
-  // of 512 27.1 / 29.1; 32 and 8 heads of 128, 16 of 400 76 / 69, 8 of 512 54 / 54,
-  // 4 of 1024 80 / 90).  At most 128 rows leave the second tile empty.
+  // 16 heads of 64, 16 sequences of 400 tokens 46.5 / 40.2, 8 of 1024 59.4 / 55.6,
+  // 6 of 1300 79.8 / 71.7, 4 of 2000 89.5 / 92.0; 32 and 8 heads of 128, 16 of 400
+  // 82.4 / 65.1, 8 of 512 58.0 / 52.0, 4 of 1300 107.8 / 104.7, 4 of 1500
+  // 123.7 / 131.2, 2 of 2000 102.2 / 121.4).  At most 128 rows leave the second
+  // tile empty.
   const bool pair =
-      static_cast<int64_t>(a->q_tokens) * p.gp > 128ll * a->batch && a->k_tokens >= 512ll * a->batch;
+      static_cast<int64_t>(a->q_tokens) * p.gp > 128ll * a->batch && a->k_tokens >= 1400ll * a->batch;
   p.cu_k = a->cu_k;
   p.k = a->k;
   p.v = a->v;

@@ -22,9 +22,10 @@
 // the request lengths on the device, so ragged lengths, long prompts and a
 // single long context load every SM alike.  A cut inside a short unit moves to
 // its nearer end (always to its start: 39 instead of 33 us for 4 requests of up
-// to 512 tokens behind 2000 keys).  A unit that a cut divides leaves fp32 partials (maximum,
-// sum, unnormalised output) in the workspace, and the worker that begins it a
-// note of where they are; a second kernel joins them, in the order of the keys.
+// to 512 tokens behind 2000 keys).  A unit that a cut divides leaves fp32
+// partials (maximum, sum, unnormalised output) in the workspace, and the worker
+// that begins it a note of where they are; a second kernel joins them, in the
+// order of the keys.
 // (Joined by the worker that arrives last instead, a CTA read up to a megabyte
 // on its own: one request of 16 drafted tokens on 8000 keys 52 us, 25 us with
 // the second kernel; 8 requests of one token on 2000 keys 31 and 21 us.)
@@ -40,10 +41,10 @@
 // the tensor pipe and on the exponential unit; P V starts on the first 64 keys
 // while the exponentials of the others are computed.  (With two tiles of 64 the
 // issue of the products bounds PAIR, with or without a softmax: 565 us where
-// this takes 490, at one prompt of 8192 tokens, 32 and 8 heads of 128.)  The output is rescaled only
-// when a row's maximum grows by more than 8 (in powers of two): a stale base
-// keeps probabilities below 2^8, which the 16-bit types and the fp32 sums hold
-// without loss.
+// this takes 490, at one prompt of 8192 tokens, 32 and 8 heads of 128.)  The
+// output is rescaled only when a row's maximum grows by more than 8 (in powers of
+// two): a stale base keeps probabilities below 2^8, which the 16-bit types and
+// the fp32 sums hold without loss.
 //
 // What bounds it.  Long prompts: per 128 keys and 128 rows at head_dim 128 the
 // tensor pipe takes 1100 cycles and the exponential unit 1024, and the chain
@@ -334,9 +335,9 @@ SVD_DEV long long steps_before(const AttnParams& p, const AttnSeq& s, int w, int
 // On the line a unit is kUnitCost and its steps long: beginning and ending a
 // unit (q, the output) costs about as much as so many steps, and the early
 // tiles of a causal prompt are many units of few steps (measured: without it
-// the CTAs that got those finished 100 us after the others at 8192 tokens; 1, 2
-// and 4 for pairs: chunks behind 5600 keys 86, 75, 70 us; for the others
-// 64-request decoding 91, 84, 87 us).
+// the CTAs that got those finished 100 us after the others at 8192 tokens; 3, 4
+// and 6 for pairs: chunks behind 5600 keys 64, 65, 69 us, 2 prompts of 2000 tokens
+// 110, 103, 103; 1, 2 and 3 for the others: 64-request decoding 91, 84, 86 us).
 template <bool PAIR>
 constexpr int kUnitCost = PAIR ? 4 : 2;
 

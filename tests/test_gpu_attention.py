@@ -70,6 +70,26 @@ def test_prompt_matches_the_formula(cuda_device, att, lq, lk, h, hk, d, dtype, c
     _status(cuda_device)
 
 
+def _behind(t, rows):
+    """`t` with `rows` rows of NaN behind it, which no sequence holds."""
+    return torch.cat([t, torch.full((rows, *t.shape[1:]), float("nan"), dtype=t.dtype, device=t.device)])
+
+
+@pytest.mark.parametrize("lq,lk,h,hk,d,dtype", PROMPTS)
+@pytest.mark.parametrize("causal,scale", [(True, None), (False, None), (True, -0.05), (False, 0.0)])
+def test_prompt_in_long_tensors(cuda_device, att, lq, lk, h, hk, d, dtype, causal, scale):
+    """The tiles for long walks over the keys are taken by the tensors' lengths."""
+    lk = lq if lk is None else lk
+    q, k, v = _qkv(sum(lq) + d, sum(lq), sum(lk), h, hk, d, dtype)
+    want, mag, tiny = ref.prompt(q, k, v, lq, lk, causal, scale)
+    k, v = _behind(k, 1500 * len(lq)), _behind(v, 1500 * len(lq))
+    cq, ck = ref.cumulative(lq, cuda_device), ref.cumulative(lk, cuda_device)
+    outs = [att.prompt_attention(q, k, v, cq, ck, causal=causal, scale=scale) for _ in range(2)]
+    _status(cuda_device)
+    ref.check(outs[0], want, mag, tiny, dtype, f"{lq} {lk}")
+    assert torch.equal(*outs)
+
+
 @pytest.mark.parametrize("scale", [0.0, 0.02, 1.0, -0.125])
 def test_prompt_scale(cuda_device, att, scale):
     lq = [140, 65]
@@ -554,15 +574,20 @@ def test_steps_through_the_cache_match_one_prompt(cuda_device, att):
     ([127, 50, 1949], [127, 0, 1949], 12, 4, 128, F16),                          # no keys between two long walks
     ([60, 1, 40, 7, 900], [0, 0, 0, 0, 5000], 8, 2, 64, BF16),
     ([300] + [2] * 40 + [500], [900] + [600] * 40 + [500], 4, 1, 128, BF16),     # second row tiles of nobody, one after another
+    ([900] + [2] * 20 + [2000], [2500] + [1400] * 20 + [2000], 4, 1, 128, BF16),
 ])
 def test_prompt_units_without_rows_or_keys(cuda_device, att, lq, lk, h, hk, d, dtype, causal):
     """Units that have nothing for one or both row tiles, between units that have; the same every time."""
     q, k, v = _qkv(sum(lk) + d, sum(lq), sum(lk), h, hk, d, dtype)
     cq, ck = ref.cumulative(lq, cuda_device), ref.cumulative(lk, cuda_device)
+    want = ref.prompt(q, k, v, lq, lk, causal)
+    far = [_behind(t, 1500 * len(lq)) for t in (k, v)]
     outs = [att.prompt_attention(q, k, v, cq, ck, causal=causal) for _ in range(8)]
+    more = [att.prompt_attention(q, *far, cq, ck, causal=causal) for _ in range(8)]
     _status(cuda_device)
-    ref.check(outs[0], *ref.prompt(q, k, v, lq, lk, causal), dtype, f"{lq} {lk}")
-    assert all(torch.equal(o, outs[0]) for o in outs)
+    for got in (outs, more):
+        ref.check(got[0], *want, dtype, f"{lq} {lk}")
+        assert all(torch.equal(o, got[0]) for o in got)
 
 
 # ----------------------------------------------------------------- refusals
