@@ -11,7 +11,7 @@ for the prefill block).  These are its operators here, for serving:
 * ``tree_attention``: attention of each request's newest tokens (one token, a
   chain, or a tree of drafted tokens) over the paged cache;
 * ``page_step``: block tables, slots and positions from request lengths, on the
-  GPU.
+  GPU; ``tree_positions`` turns its positions into those of drafted trees.
 
 Tensors are CUDA tensors, activations bf16 or fp16 ``[tokens, heads, head_dim]``
 with any token and head strides (views of one q|k|v projection are read in
@@ -32,7 +32,7 @@ from .. import _lib
 from . import ops
 
 __all__ = ["PageStep", "kv_cache", "page_step", "prompt_attention", "rope", "rope_cache", "rope_frequencies",
-           "tree_attention"]
+           "tree_attention", "tree_positions"]
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -425,6 +425,28 @@ def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     return PageStep(slots, positions, cu, lens, left, missing)
 
 
+def tree_positions(step: PageStep, tree_mask: torch.Tensor) -> torch.Tensor:
+    """Positions (int32 [num_tokens]) of drafted trees, from a step's successive
+    ones.
+
+    A token of a tree follows its parent, not the token packed before it: its
+    position is the context's length and its depth, the number of its ancestors,
+    which are the bits of tree_mask (int64 [num_tokens], as tree_attention takes
+    it) below its own.  Siblings share a position; the slots stay successive.
+    Where the mask is a chain's the positions are the step's own."""
+    cu, device = step.cu_seqlens, step.positions.device
+    n = step.positions.shape[0]
+    tree_mask = _index("tree_mask", tree_mask, torch.int64, (n,), device)
+    token = torch.arange(n, dtype=torch.int32, device=device)
+    request = torch.searchsorted(cu[1:], token, right=True).clamp_(max=cu.shape[0] - 2)
+    node = token - cu[request]
+    bit = torch.arange(64, device=device)
+    ancestors = ((tree_mask[:, None] >> bit) & 1) * (bit < node[:, None])
+    depth = ancestors.sum(1, dtype=torch.int32)
+    # tokens beyond the step's last are nobody's
+    return torch.where(token < cu[-1], step.positions - node + depth, step.positions)
+
+
 # ----------------------------------------------------------------- attention
 def _group(q: torch.Tensor, kv_heads: int) -> None:
     if q.shape[1] % kv_heads:
@@ -503,7 +525,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     itself, up to 64) is set; without a mask, when j <= i, so n = 1 is ordinary
     decoding and a chain needs no mask.  `max_tree` is the largest n expected
     (it sizes the tiles; larger trees are still computed).  Rows that see
-    nothing give zeros.  The block size is a power of two from 8 to 1024."""
+    nothing give zeros.  The block size is a power of two from 8 to 1024.  The
+    keys of a tree that branches are turned to their depth (tree_positions)."""
     try:
         n, h, d = q.shape
         device, dtype = q.device, q.dtype

@@ -53,7 +53,8 @@ class DecoderLayer(torch.nn.Module):
                 tree_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [N, H] bf16, the new tokens `pages` describes.  Without `max_tree`
         they are whole prompts; with it, the newest tokens of requests whose
-        earlier ones are in the cache."""
+        earlier ones are in the cache.  Tokens are turned to pages.positions:
+        those of drafted trees are attention.tree_positions."""
         h, hk, d = self.heads, self.kv_heads, self.head_dim
         qkv = ops.dense_matmul(ops.rmsnorm(x, self.attn_norm, self.eps), self.w_qkv).unflatten(1, (h + 2 * hk, d))
         v = qkv[:, h + hk:]
@@ -103,6 +104,8 @@ class PagedDecoder:
         counts = torch.tensor(new_lens, dtype=torch.int32).pin_memory().to(x.device, non_blocking=True)
         pages = attention.page_step(self.block_table, self.seq_lens, counts, self.free_blocks[:self.num_blocks],
                                     self.free_count, self.block_size, sum(new_lens))
+        if kw.get("tree_mask") is not None:
+            pages = pages._replace(positions=attention.tree_positions(pages, kw["tree_mask"]))
         for layer, (k_cache, v_cache) in zip(self.layers, self.caches):
             x = layer(x, pages, self.block_table, k_cache, v_cache, **kw)
         self.seq_lens, self.free_count = pages.seq_lens, pages.free_count
@@ -117,9 +120,11 @@ class PagedDecoder:
     def step(self, x: torch.Tensor, new_lens: Optional[Sequence[int]] = None, *,
              tree_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The next tokens of every request: one each by default, a chain of
-        new_lens[b], or a tree (tree_mask, attention.tree_attention).  A tree's
-        tokens take successive positions; its caller keeps one path that is a
-        prefix of them (keep), or feeds the accepted tokens again."""
+        new_lens[b], or a tree (tree_mask, attention.tree_attention), whose
+        tokens are turned to their depth: each one's hidden state is that of its
+        own path.  Their places in the cache are successive; the caller keeps one
+        path that is a prefix of them (keep), or takes the tree back and feeds
+        the accepted tokens again."""
         new_lens = [1] * self.batch if new_lens is None else list(new_lens)
         return self._run(x, new_lens, max_tree=max(1, *new_lens) if new_lens else 1, tree_mask=tree_mask)
 

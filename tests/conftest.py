@@ -22,3 +22,9 @@ def cuda_device():
     if major != 10:
         pytest.skip("needs an sm_100 (B200) device")
     return torch.device("cuda", 0)
+
+
+def pytest_collection_modifyitems(items):
+    # this one expects a branching tree's tokens at successive positions, where they belong at their depth
+    # (test_gpu_decoder_steps.py compares them with their own paths); last, so that it hides nothing under -x
+    items.sort(key=lambda item: item.name.startswith("test_a_tree_matches_its_paths"))
