@@ -13,7 +13,8 @@ language-model head belong to the caller.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+import itertools
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -73,8 +74,12 @@ class DecoderLayer(torch.nn.Module):
 class PagedDecoder:
     """A stack of DecoderLayers, its caches and the tables of `batch` requests.
 
-    Lengths, tables and the free list live on the GPU; a step's token counts
-    come from the host, so no call waits for the device."""
+    Lengths, tables and the free list live on the GPU, in tensors that every call
+    updates in place; a step's token counts come from the host, so no call waits
+    for the device.  A step can therefore be captured in a CUDA graph (one step
+    on the capturing stream before it sets up weights and workspaces): each
+    replay goes on from where the requests are, for the counts that it was
+    captured with."""
 
     def __init__(self, layers: Sequence[DecoderLayer], batch: int, num_blocks: int, max_length: int, *,
                  block_size: int = 16, device="cuda"):
@@ -101,16 +106,31 @@ class PagedDecoder:
             raise ValueError(f"new_lens must give {self.batch} counts that sum to x's {x.shape[0]} rows")
         if not x.shape[0]:
             return x
-        counts = torch.tensor(new_lens, dtype=torch.int32).pin_memory().to(x.device, non_blocking=True)
-        pages = attention.page_step(self.block_table, self.seq_lens, counts, self.free_blocks[:self.num_blocks],
+        pages = attention.page_step(self.block_table, self.seq_lens, self._counts(new_lens), self.free_blocks[:self.num_blocks],
                                     self.free_count, self.block_size, sum(new_lens))
         if kw.get("tree_mask") is not None:
             pages = pages._replace(positions=attention.tree_positions(pages, kw["tree_mask"]))
         for layer, (k_cache, v_cache) in zip(self.layers, self.caches):
             x = layer(x, pages, self.block_table, k_cache, v_cache, **kw)
-        self.seq_lens, self.free_count = pages.seq_lens, pages.free_count
-        self.missing = torch.maximum(self.missing, pages.missing)
+        self.seq_lens.copy_(pages.seq_lens)
+        self.free_count.copy_(pages.free_count)
+        torch.maximum(self.missing, pages.missing, out=self.missing)
         return x
+
+    def _counts(self, new_lens: List[int]) -> torch.Tensor:
+        """`new_lens` on the device."""
+        device = self.seq_lens.device
+        if len(set(new_lens)) == 1:
+            return torch.full((self.batch,), new_lens[0], dtype=torch.int32, device=device)
+        if not torch.cuda.is_current_stream_capturing():
+            return torch.tensor(new_lens, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
+        # a captured copy would read host memory at every replay, long after this call: filled in place, run by run
+        counts, at = torch.empty(self.batch, dtype=torch.int32, device=device), 0
+        for n, run in itertools.groupby(new_lens):
+            length = len(list(run))
+            counts[at:at + length].fill_(n)
+            at += length
+        return counts
 
     def prefill(self, x: torch.Tensor, lens: Sequence[int]) -> torch.Tensor:
         """Whole prompts: x [sum(lens), H] bf16, requests in order, all of them
@@ -140,8 +160,8 @@ class PagedDecoder:
         place = torch.where(flat, self.free_count + flat.cumsum(0) - 1, self.num_blocks)
         self.free_blocks[place] = self.block_table.flatten()
         self.block_table[:] = torch.where(freed, -1, self.block_table)
-        self.free_count = (self.free_count + flat.sum(dtype=torch.int32)).to(torch.int32)
-        self.seq_lens = lens
+        self.free_count += flat.sum(dtype=torch.int32)
+        self.seq_lens.copy_(lens)
 
     def check(self) -> None:
         """Waits for the device; raises if the cache ran out of blocks, or a kernel reported an error."""

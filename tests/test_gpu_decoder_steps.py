@@ -52,3 +52,49 @@ def test_every_tree_token_is_its_own_path(cuda_device, model):
     dec.keep(torch.tensor(contexts, dtype=torch.int32, device="cuda"))
     again = dec.step(xs[0][contexts[0]:][path], [len(path), 0])
     plain._close(again, y[path].double(), "the path as a chain")
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [3, 1, 2], [2, 2, 0]])
+def test_replays_of_a_captured_step_go_on(cuda_device, model, news):
+    """Twenty replays, into new blocks, against the plain decoder and against eager steps, with tokens taken back
+    between them."""
+    from svdflash_b200.models import PagedDecoder
+    layers, weights, inv_freq = model
+    lens, replays = [33, 1, 150], 20
+    xs = [_hidden(50 + b, n + k * (replays + 1)) for b, (n, k) in enumerate(zip(lens, news))]
+
+    def tokens(step):
+        return torch.cat([x[n + k * step:n + k * (step + 1)] for x, n, k in zip(xs, lens, news)])
+    decs = [PagedDecoder(layers, 3, 40, 256) for _ in range(2)]
+    outs = [[o] for o in decs[0].prefill(torch.cat([x[:n] for x, n in zip(xs, lens)]), lens).split(lens)]
+    decs[1].prefill(torch.cat([x[:n] for x, n in zip(xs, lens)]), lens)
+    feed = tokens(0)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        first = decs[0].step(feed, news)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            last = decs[0].step(feed, news)
+    decs[1].step(feed, news)
+    for o, part in zip(outs, first.split(news)):
+        o.append(part)
+    junk = _hidden(60, sum(news))
+    for i in range(1, replays + 1):
+        if i % 7 == 0:                                  # a draft that is taken back
+            held = decs[0].seq_lens.clone()
+            feed.copy_(junk)
+            graph.replay()
+            decs[0].keep(held)
+        feed.copy_(tokens(i))
+        graph.replay()
+        for o, part in zip(outs, last.clone().split(news)):
+            o.append(part)
+        decs[1].step(tokens(i), news)
+    decs[0].check()
+    total = [n + k * (replays + 1) for n, k in zip(lens, news)]
+    assert decs[0].seq_lens.tolist() == decs[1].seq_lens.tolist() == total
+    assert decs[0].free_count.tolist() == decs[1].free_count.tolist() == [40 - sum(-(-t // 16) for t in total)]
+    assert (decs[0].block_table >= 0).sum().item() == sum(-(-t // 16) for t in total)
+    for b in range(3):
+        plain._close(torch.cat(outs[b]), _alone(xs[b], weights, inv_freq), f"request {b}")
