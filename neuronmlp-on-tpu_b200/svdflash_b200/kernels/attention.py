@@ -392,7 +392,9 @@ def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     block_table are left as they are: a caller keeps the returned seq_lens and
     free_count for the next step, and frees blocks by writing them behind
     free_count.  `missing` above zero means that the free list ran out: those
-    blocks' entries and slots are -1."""
+    blocks' entries and slots are -1.  A request's tokens beyond the table's
+    W * block_size places get slot -1 too; they count in seq_lens, which tells
+    them, and not in `missing`."""
     try:
         b, width = block_table.shape
         index, one = block_table.get_device(), (1,)

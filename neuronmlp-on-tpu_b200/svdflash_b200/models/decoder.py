@@ -99,6 +99,8 @@ class PagedDecoder:
         self.free_count = torch.tensor([num_blocks], dtype=torch.int32, device=dev)
         self.num_blocks = num_blocks
         self.missing = torch.zeros(1, dtype=torch.int32, device=dev)
+        # the longest that each request has been: page_step drops what lies beyond the table's width
+        self.longest = torch.zeros(batch, dtype=torch.int32, device=dev)
 
     def _run(self, x: torch.Tensor, new_lens: Sequence[int], **kw) -> torch.Tensor:
         new_lens = [int(n) for n in new_lens]
@@ -115,6 +117,7 @@ class PagedDecoder:
         self.seq_lens.copy_(pages.seq_lens)
         self.free_count.copy_(pages.free_count)
         torch.maximum(self.missing, pages.missing, out=self.missing)
+        torch.maximum(self.longest, pages.seq_lens, out=self.longest)
         return x
 
     def _counts(self, new_lens: List[int]) -> torch.Tensor:
@@ -164,8 +167,12 @@ class PagedDecoder:
         self.seq_lens.copy_(lens)
 
     def check(self) -> None:
-        """Waits for the device; raises if the cache ran out of blocks, or a kernel reported an error."""
-        short = int(self.missing.item())
+        """Waits for the device; raises if the cache ran out of blocks, if a request outgrew its table since the
+        decoder was made, or if a kernel reported an error."""
+        short, longest = int(self.missing.item()), int(self.longest.max().item())
         ops.check_device_status(self.seq_lens.device)
+        places = self.block_table.shape[1] * self.block_size
+        if longest > places:
+            raise RuntimeError(f"a request of {longest} tokens outgrew its table of {places}: tokens were dropped")
         if short:
             raise RuntimeError(f"the cache had {short} blocks too few: tokens were dropped")

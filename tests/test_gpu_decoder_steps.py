@@ -98,3 +98,23 @@ def test_replays_of_a_captured_step_go_on(cuda_device, model, news):
     assert (decs[0].block_table >= 0).sum().item() == sum(-(-t // 16) for t in total)
     for b in range(3):
         plain._close(torch.cat(outs[b]), _alone(xs[b], weights, inv_freq), f"request {b}")
+
+
+@pytest.mark.parametrize("how", ["prefill", "step", "chain"])
+def test_a_request_that_outgrows_its_table_is_reported(cuda_device, model, how):
+    from svdflash_b200.models import PagedDecoder
+    layers, _, _ = model
+    dec = PagedDecoder(layers, 2, 12, 33)                # three blocks of 16: 48 tokens a request
+    x = _hidden(70, 100)
+    dec.prefill(x[:48 + 5], [48, 5])
+    dec.check()                                          # full, and no more
+    if how == "prefill":
+        dec = PagedDecoder(layers, 2, 12, 33)
+        dec.prefill(x[:49 + 5], [49, 5])
+    elif how == "step":
+        dec.step(x[:2])
+    else:
+        dec.step(x[:9], [9, 0])
+        dec.keep(torch.tensor([40, 5], dtype=torch.int32, device="cuda"))   # what was dropped stays reported
+    with pytest.raises(RuntimeError, match="outgrew its table of 48"):
+        dec.check()
