@@ -101,6 +101,8 @@ class PagedDecoder:
         self.missing = torch.zeros(1, dtype=torch.int32, device=dev)
         # the longest that each request has been: page_step drops what lies beyond the table's width
         self.longest = torch.zeros(batch, dtype=torch.int32, device=dev)
+        # tokens that a request held when prefill was given more of it
+        self.prefilled = torch.zeros(batch, dtype=torch.int32, device=dev)
 
     def _run(self, x: torch.Tensor, new_lens: Sequence[int], **kw) -> torch.Tensor:
         new_lens = [int(n) for n in new_lens]
@@ -108,12 +110,15 @@ class PagedDecoder:
             raise ValueError(f"new_lens must give {self.batch} counts that sum to x's {x.shape[0]} rows")
         if not x.shape[0]:
             return x
-        pages = attention.page_step(self.block_table, self.seq_lens, self._counts(new_lens), self.free_blocks[:self.num_blocks],
+        counts = self._counts(new_lens)
+        pages = attention.page_step(self.block_table, self.seq_lens, counts, self.free_blocks[:self.num_blocks],
                                     self.free_count, self.block_size, sum(new_lens))
         if kw.get("tree_mask") is not None:
             pages = pages._replace(positions=attention.tree_positions(pages, kw["tree_mask"]))
         for layer, (k_cache, v_cache) in zip(self.layers, self.caches):
             x = layer(x, pages, self.block_table, k_cache, v_cache, **kw)
+        if "max_tree" not in kw:  # prompt attention sees the call's own tokens only
+            torch.maximum(self.prefilled, self.seq_lens * (counts > 0), out=self.prefilled)
         self.seq_lens.copy_(pages.seq_lens)
         self.free_count.copy_(pages.free_count)
         torch.maximum(self.missing, pages.missing, out=self.missing)
@@ -136,8 +141,9 @@ class PagedDecoder:
         return counts
 
     def prefill(self, x: torch.Tensor, lens: Sequence[int]) -> torch.Tensor:
-        """Whole prompts: x [sum(lens), H] bf16, requests in order, all of them
-        empty before.  Returns the hidden states of every token."""
+        """Whole prompts: x [sum(lens), H] bf16, requests in order; those that get
+        tokens are empty before (check() reports one that was not: step takes
+        the chunks of a prompt).  Returns the hidden states of every token."""
         return self._run(x, lens)
 
     def step(self, x: torch.Tensor, new_lens: Optional[Sequence[int]] = None, *,
@@ -167,12 +173,15 @@ class PagedDecoder:
         self.seq_lens.copy_(lens)
 
     def check(self) -> None:
-        """Waits for the device; raises if the cache ran out of blocks, if a request outgrew its table since the
-        decoder was made, or if a kernel reported an error."""
+        """Waits for the device; raises if, since the decoder was made, the cache ran out of blocks, a request outgrew
+        its table or prefill was given one that held tokens, or if a kernel reported an error."""
         short, longest = int(self.missing.item()), int(self.longest.max().item())
+        before = int(self.prefilled.max().item())
         ops.check_device_status(self.seq_lens.device)
         places = self.block_table.shape[1] * self.block_size
         if longest > places:
             raise RuntimeError(f"a request of {longest} tokens outgrew its table of {places}: tokens were dropped")
+        if before:
+            raise RuntimeError(f"prefill was given a request that held {before} tokens: its new ones did not see them")
         if short:
             raise RuntimeError(f"the cache had {short} blocks too few: tokens were dropped")

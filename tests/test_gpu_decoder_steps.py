@@ -118,3 +118,24 @@ def test_a_request_that_outgrows_its_table_is_reported(cuda_device, model, how):
         dec.keep(torch.tensor([40, 5], dtype=torch.int32, device="cuda"))   # what was dropped stays reported
     with pytest.raises(RuntimeError, match="outgrew its table of 48"):
         dec.check()
+
+
+def test_prefill_of_a_request_that_holds_tokens_is_reported(cuda_device, model):
+    from svdflash_b200.models import PagedDecoder
+    layers, weights, inv_freq = model
+    x = _hidden(80, 60)
+    dec = PagedDecoder(layers, 2, 12, 64)
+    dec.prefill(x[:20], [20, 0])
+    y = dec.prefill(x[20:50], [0, 30])                   # one request after another
+    dec.check()
+    plain._close(y, _alone(x[20:50], weights, inv_freq), "the second request")
+    dec.keep(torch.zeros(2, dtype=torch.int32, device="cuda"))
+    y = dec.prefill(x[:50], [40, 10])                    # new requests in the places of old ones
+    dec.check()
+    plain._close(y[:40], _alone(x[:40], weights, inv_freq), "a new request")
+    z = dec.step(x[40:50], [10, 0])                      # a prompt's second chunk
+    dec.check()
+    plain._close(z, _alone(x[:50], weights, inv_freq)[40:], "the second chunk")
+    dec.prefill(x[50:60], [0, 10])
+    with pytest.raises(RuntimeError, match="held 10 tokens"):
+        dec.check()
