@@ -630,8 +630,9 @@ int svdmlp_prompt_attention(const svdmlp_prompt_args* args, void* stream);
  * cache, the newest n being its tree.  Every row sees the context (the first
  * lens - n); in the tree, row i sees tree token j when bit j of mask[row] is
  * set, or, with mask NULL, when j <= i (a chain; n = 1 is ordinary decoding).
- * A mask names the first 64 tree tokens only.  max_tree, the largest n the
- * caller expects, sizes the tiles; larger trees are still computed. */
+ * max_tree, the largest n the caller expects, sizes the tiles; larger trees are
+ * still computed, but a mask names the first 64 tree tokens only: with one
+ * max_tree is at most 64. */
 typedef struct svdmlp_tree_args {
   int32_t dtype, batch, tokens, q_heads, kv_heads, head_dim;
   int32_t block_size, num_blocks, table_width, max_tree;

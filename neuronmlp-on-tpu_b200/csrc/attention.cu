@@ -325,6 +325,7 @@ static int tree_impl(const svdmlp_tree_args* a, cudaStream_t s) {
   SVD_CHECK(check_heads(a->dtype, a->q_heads, a->kv_heads, a->head_dim, a->scale));
   if (a->block_size < 8 || a->block_size > 1024 || (a->block_size & (a->block_size - 1)) != 0)
     return SVDMLP_ERR_SHAPE_MISMATCH;
+  if (a->mask && a->max_tree > 64) return SVDMLP_ERR_SHAPE_MISMATCH;  // a row's mask has a bit for each of 64 tokens
   const int64_t inside = static_cast<int64_t>(a->kv_heads) * a->block_size * a->head_dim;
   if (a->k_block < inside || a->v_block < inside || a->ld_table < a->table_width) return SVDMLP_ERR_SHAPE_MISMATCH;
   if (!rows_aligned(a->q, a->q_token, a->q_head) || !rows_aligned(a->k_cache, a->k_block, 0) ||

@@ -44,6 +44,7 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch.cuda.current_device
 _PLAIN = torch.contiguous_format
+_MASK_BITS = 64  # tree tokens that a row's mask names
 
 
 def _refuse_dtype(t) -> None:
@@ -442,7 +443,7 @@ def tree_positions(step: PageStep, tree_mask: torch.Tensor) -> torch.Tensor:
     token = torch.arange(n, dtype=torch.int32, device=device)
     request = torch.searchsorted(cu[1:], token, right=True).clamp_(max=cu.shape[0] - 2)
     node = token - cu[request]
-    bit = torch.arange(64, device=device)
+    bit = torch.arange(_MASK_BITS, device=device)
     ancestors = ((tree_mask[:, None] >> bit) & 1) * (bit < node[:, None])
     depth = ancestors.sum(1, dtype=torch.int32)
     # tokens beyond the step's last are nobody's
@@ -524,9 +525,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     names (int32 [B, W]); the newest n are its tree, in the rows' order.  Every
     row sees the seq_lens[b] - n tokens of the context.  In the tree, row i sees
     token j when bit j of tree_mask[row] (int64 [N]: a token's ancestors and
-    itself, up to 64) is set; without a mask, when j <= i, so n = 1 is ordinary
-    decoding and a chain needs no mask.  `max_tree` is the largest n expected
-    (it sizes the tiles; larger trees are still computed).  Rows that see
+    itself) is set; without a mask, when j <= i, so n = 1 is ordinary decoding
+    and a chain needs no mask.  `max_tree` is the largest n expected: it sizes
+    the tiles, and larger trees are still computed, but a mask names the first
+    64 tokens only, so with one max_tree is at most 64.  Rows that see
     nothing give zeros.  The block size is a power of two from 8 to 1024.  The
     keys of a tree that branches are turned to their depth (tree_positions)."""
     try:
@@ -559,6 +561,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         tree_mask = _index("tree_mask", tree_mask, torch.int64, (n,), device)
         mask_ptr = tree_mask.data_ptr()
     ops._positive("max_tree", max_tree)
+    if mask_ptr and max_tree > _MASK_BITS:
+        raise ValueError(f"tree_mask names {_MASK_BITS} tokens of a request, max_tree is {max_tree}")
     scale = _scale(scale, d)
     out = torch.empty_like(q, memory_format=_PLAIN) if out is None else _output(out, q)
     if n == 0:

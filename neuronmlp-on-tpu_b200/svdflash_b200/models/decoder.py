@@ -155,6 +155,8 @@ class PagedDecoder:
         path that is a prefix of them (keep), or takes the tree back and feeds
         the accepted tokens again."""
         new_lens = [1] * self.batch if new_lens is None else list(new_lens)
+        if tree_mask is not None and max(new_lens, default=0) > 64:
+            raise ValueError(f"a tree has at most 64 tokens, got {max(new_lens)}")
         return self._run(x, new_lens, max_tree=max(1, *new_lens) if new_lens else 1, tree_mask=tree_mask)
 
     def keep(self, lens: torch.Tensor) -> None:

@@ -139,3 +139,18 @@ def test_prefill_of_a_request_that_holds_tokens_is_reported(cuda_device, model):
     dec.prefill(x[50:60], [0, 10])
     with pytest.raises(RuntimeError, match="held 10 tokens"):
         dec.check()
+
+
+def test_a_masked_tree_of_more_than_64_tokens_is_refused(cuda_device, model):
+    """A row's mask has no bits for the tokens behind the 64th: they would not even see themselves."""
+    from svdflash_b200.models import PagedDecoder
+    layers, _, _ = model
+    dec = PagedDecoder(layers, 1, 12, 160)
+    dec.prefill(_hidden(90, 10), [10])
+    mask = torch.ones(70, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="at most 64"):
+        dec.step(_hidden(91, 70), [70], tree_mask=mask)
+    assert dec.seq_lens.tolist() == [10]
+    dec.step(_hidden(91, 64), [64], tree_mask=mask[:64])
+    dec.step(_hidden(91, 70), [70])                      # a chain has no such end
+    dec.check()
