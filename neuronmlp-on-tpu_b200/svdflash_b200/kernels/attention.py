@@ -169,9 +169,41 @@ def _output(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
         raise TypeError("out must have the inputs' dtype")
     if not _vector_rows(out, out.stride()):
         raise ValueError("out must have 16-byte aligned rows")
-    if out.data_ptr() == q.data_ptr() and q.numel():
-        raise ValueError("out must not overlap the inputs")
     return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors [tokens, heads, elements] of one type with unit stride in the last dimension share a place."""
+    (a_n, a_heads, a_row), (b_n, b_heads, b_row) = a.shape, b.shape
+    a_token, b_token = (t.stride(0) if t.shape[0] > 1 else 0 for t in (a, b))
+    a_head, b_head = (t.stride(1) if t.shape[1] > 1 else 0 for t in (a, b))
+    ahead = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    a_heads, b_heads = (a_heads - 1) * a_head + a_row, (b_heads - 1) * b_head + b_row      # places of a token's heads
+    a_tokens, b_tokens = (a_n - 1) * a_token + a_row, (b_n - 1) * b_token + b_row          # of a head's tokens
+    if a_tokens + a_heads - a_row <= ahead or b_tokens + b_heads - b_row <= -ahead:
+        return False
+    # views of one buffer that lie side by side or take turns: b at the same place between two rows, between two
+    # tokens or between two heads of a
+    for period, mine, other in ((math.gcd(a_token, b_token, a_head, b_head), a_row, b_row),
+                                (a_token if a_token == b_token else 0, a_heads, b_heads),
+                                (a_head if a_head == b_head else 0, a_tokens, b_tokens)):
+        if period and mine <= ahead % period <= period - other:
+            return False
+    # whatever else: the rows of both in the order of their places, each against the ends of the other's before it
+    a_at, b_at = ((start + torch.arange(t.shape[0])[:, None] * token + torch.arange(t.shape[1]) * head).flatten()
+                  for t, start, token, head in ((a, 0, a_token, a_head), (b, ahead, b_token, b_head)))
+    places, order = torch.cat((a_at, b_at)).sort(stable=True)
+    of_a = order < a_at.numel()
+    before = torch.iinfo(torch.int64).min
+    a_end = torch.where(of_a, places + a_row, before).cummax(0).values
+    b_end = torch.where(of_a, before, places + b_row).cummax(0).values
+    return bool((torch.where(of_a, b_end, a_end) > places).any())
+
+
+def _apart(out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Refuses an `out` that shares memory with inputs that the kernels read while they write it."""
+    if out.numel() and any(t.numel() and _overlap(out, t) for t in inputs):
+        raise ValueError("out must not overlap the inputs")
 
 
 def _call(fn, args: bytes, device: torch.device, what: str) -> None:
@@ -495,12 +527,15 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if cu_k.shape != cu_q.shape:
             raise ValueError("cu_q and cu_k must have matching shapes")
     scale = _scale(scale, d)
-    out = torch.empty_like(q, memory_format=_PLAIN) if out is None else _output(out, q)
+    given = out is not None
+    out = _output(out, q) if given else torch.empty_like(q, memory_format=_PLAIN)
     if nq == 0:
         return out
     if nk == 0:
         return out.zero_()
     q, k, v = _rows(q), _rows(k), _rows(v)
+    if given:
+        _apart(out, q, k, v)
     ws = _workspace(device, d)
     q_token, q_head, _ = q.stride()
     k_token, k_head, _ = k.stride()
@@ -564,10 +599,13 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if mask_ptr and max_tree > _MASK_BITS:
         raise ValueError(f"tree_mask names {_MASK_BITS} tokens of a request, max_tree is {max_tree}")
     scale = _scale(scale, d)
-    out = torch.empty_like(q, memory_format=_PLAIN) if out is None else _output(out, q)
+    given = out is not None
+    out = _output(out, q) if given else torch.empty_like(q, memory_format=_PLAIN)
     if n == 0:
         return out
     q = _rows(q)
+    if given:
+        _apart(out, q, *(t.flatten(1).unsqueeze(1) for t in (k_cache, v_cache)))
     ws = _workspace(device, d)
     q_token, q_head, _ = q.stride()
     o_token, o_head, _ = out.stride()
