@@ -628,16 +628,19 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         float4 o[C][N];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float* from = partial(min(b0 + k, u.more));
-          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
-          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
+          // behind the last one: nothing seen (its output again, by a weight of 0, would turn an infinity into NaN)
+          const bool one = b0 + k <= u.more;
+          const float* from = partial(b0 + k);
+          f[k] = one ? __ldcg(from + Cfg::PART_ROWS * D + row) : -INFINITY;
+          g[k] = one ? __ldcg(from + Cfg::PART_ROWS * (D + 1) + row) : 0.f;
 #pragma unroll
           for (int n = 0; n < N; ++n)
-            o[k][n] = __ldcg(reinterpret_cast<const float4*>(from) + (warp * N + n) * Cfg::PART_ROWS + row);
+            o[k][n] = one ? __ldcg(reinterpret_cast<const float4*>(from) + (warp * N + n) * Cfg::PART_ROWS + row)
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         float top = mm;
 #pragma unroll
-        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
+        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);
         const float safe = top == -INFINITY ? 0.f : top;
         const float old = exp2_approx(mm - safe);
         mm = top;
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         for (int n = 0; n < N; ++n) acc[n] = make_float4(acc[n].x * old, acc[n].y * old, acc[n].z * old, acc[n].w * old);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float e = b0 + k <= u.more ? exp2_approx(f[k] - safe) : 0.f;
+          const float e = exp2_approx(f[k] - safe);
           ll = fmaf(e, g[k], ll);
 #pragma unroll
           for (int n = 0; n < N; ++n) {
@@ -679,10 +682,11 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         float f[C], g[C];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float* from = partial(min(b0 + k, u.more));
-          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
-          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
-          o[k] = __ldcg(reinterpret_cast<const float4*>(from + row * D) + d4);
+          const bool one = b0 + k <= u.more;
+          const float* from = partial(b0 + k);
+          f[k] = one ? __ldcg(from + Cfg::PART_ROWS * D + row) : -INFINITY;
+          g[k] = one ? __ldcg(from + Cfg::PART_ROWS * (D + 1) + row) : 0.f;
+          o[k] = one ? __ldcg(reinterpret_cast<const float4*>(from + row * D) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         float top = mm;
 #pragma unroll
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float e = b0 + k <= u.more ? exp2_approx(f[k] - safe) : 0.f;
+          const float e = exp2_approx(f[k] - safe);
           ll = fmaf(e, g[k], ll);
           acc.x = fmaf(e, o[k].x, acc.x);
           acc.y = fmaf(e, o[k].y, acc.y);
