@@ -594,11 +594,12 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
 // begins (most begin none), block rows over its rows.  Statistics and outputs of
 // several partials are in flight at a time and joined as they come, with a
 // running maximum, in the order of the keys.  Latency-bound: 5 us for 8 units of
-// 37 partials (8 key/value heads, one token on 65537 keys).
+// 37 partials (8 key/value heads, one token on 65537 keys).  Three CTAs an SM, as
+// most have nothing to join (two: 24 ragged prompts 31.1 instead of 30.2 us).
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D, bool PAIR>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, 3) attention_join_kernel(const __grid_constant__ AttnParams p) {
   using Cfg = AttnCfg<D, PAIR>;
   grid_dependency_wait();
   const int c0 = blockIdx.x;
@@ -628,19 +629,16 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         float4 o[C][N];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          // behind the last one: nothing seen (its output again, by a weight of 0, would turn an infinity into NaN)
-          const bool one = b0 + k <= u.more;
-          const float* from = partial(b0 + k);
-          f[k] = one ? __ldcg(from + Cfg::PART_ROWS * D + row) : -INFINITY;
-          g[k] = one ? __ldcg(from + Cfg::PART_ROWS * (D + 1) + row) : 0.f;
+          const float* from = partial(min(b0 + k, u.more));
+          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
+          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
 #pragma unroll
           for (int n = 0; n < N; ++n)
-            o[k][n] = one ? __ldcg(reinterpret_cast<const float4*>(from) + (warp * N + n) * Cfg::PART_ROWS + row)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
+            o[k][n] = __ldcg(reinterpret_cast<const float4*>(from) + (warp * N + n) * Cfg::PART_ROWS + row);
         }
         float top = mm;
 #pragma unroll
-        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);
+        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
         const float safe = top == -INFINITY ? 0.f : top;
         const float old = exp2_approx(mm - safe);
         mm = top;
@@ -649,14 +647,16 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         for (int n = 0; n < N; ++n) acc[n] = make_float4(acc[n].x * old, acc[n].y * old, acc[n].z * old, acc[n].w * old);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float e = exp2_approx(f[k] - safe);
-          ll = fmaf(e, g[k], ll);
+          // nothing of what lies behind the last one: by a weight of 0 an infinity would turn into NaN
+          const bool one = b0 + k <= u.more;
+          const float e = one ? exp2_approx(f[k] - safe) : 0.f;
+          ll = fmaf(e, one ? g[k] : 0.f, ll);
 #pragma unroll
           for (int n = 0; n < N; ++n) {
-            acc[n].x = fmaf(e, o[k][n].x, acc[n].x);
-            acc[n].y = fmaf(e, o[k][n].y, acc[n].y);
-            acc[n].z = fmaf(e, o[k][n].z, acc[n].z);
-            acc[n].w = fmaf(e, o[k][n].w, acc[n].w);
+            acc[n].x = fmaf(e, one ? o[k][n].x : 0.f, acc[n].x);
+            acc[n].y = fmaf(e, one ? o[k][n].y : 0.f, acc[n].y);
+            acc[n].z = fmaf(e, one ? o[k][n].z : 0.f, acc[n].z);
+            acc[n].w = fmaf(e, one ? o[k][n].w : 0.f, acc[n].w);
           }
         }
       }
@@ -682,15 +682,14 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         float f[C], g[C];
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const bool one = b0 + k <= u.more;
-          const float* from = partial(b0 + k);
-          f[k] = one ? __ldcg(from + Cfg::PART_ROWS * D + row) : -INFINITY;
-          g[k] = one ? __ldcg(from + Cfg::PART_ROWS * (D + 1) + row) : 0.f;
-          o[k] = one ? __ldcg(reinterpret_cast<const float4*>(from + row * D) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float* from = partial(min(b0 + k, u.more));
+          f[k] = __ldcg(from + Cfg::PART_ROWS * D + row);
+          g[k] = __ldcg(from + Cfg::PART_ROWS * (D + 1) + row);
+          o[k] = __ldcg(reinterpret_cast<const float4*>(from + row * D) + d4);
         }
         float top = mm;
 #pragma unroll
-        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);
+        for (int k = 0; k < C; ++k) top = fmaxf(top, f[k]);  // the last one again where there are fewer
         const float safe = top == -INFINITY ? 0.f : top;
         const float old = exp2_approx(mm - safe);
         mm = top;
@@ -698,12 +697,13 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
         acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
 #pragma unroll
         for (int k = 0; k < C; ++k) {
-          const float e = exp2_approx(f[k] - safe);
-          ll = fmaf(e, g[k], ll);
-          acc.x = fmaf(e, o[k].x, acc.x);
-          acc.y = fmaf(e, o[k].y, acc.y);
-          acc.z = fmaf(e, o[k].z, acc.z);
-          acc.w = fmaf(e, o[k].w, acc.w);
+          const bool one = b0 + k <= u.more;
+          const float e = one ? exp2_approx(f[k] - safe) : 0.f;
+          ll = fmaf(e, one ? g[k] : 0.f, ll);
+          acc.x = fmaf(e, one ? o[k].x : 0.f, acc.x);
+          acc.y = fmaf(e, one ? o[k].y : 0.f, acc.y);
+          acc.z = fmaf(e, one ? o[k].z : 0.f, acc.z);
+          acc.w = fmaf(e, one ? o[k].w : 0.f, acc.w);
         }
       }
       const float iv = ll == 0.f ? 0.f : 1.f / ll;
