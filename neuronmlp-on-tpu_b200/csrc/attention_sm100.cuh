@@ -402,47 +402,150 @@ struct AttnWalk {
 };
 
 // ------------------------------------------------------- the row-wise path
-// The output of one row over the keys [j_lo, j_hi) of its segment, a warp per
-// row, keys that the row does not see left out altogether.  Taken only where
-// the tiled product gave a value that is not finite: the product multiplies
-// every value in a tile, and 0 * inf in a masked place would reach rows that
-// do not see it.  `base` is the row's maximum, in the exponent's units.
-template <typename T, int D>
-__device__ __noinline__ void attn_row(const AttnParams& p, const AttnSeq& s, int b, int token, int head, int kv_head,
-                                      int j_lo, int j_hi, float base, float (&o)[D / 32]) {
-  constexpr int E = D / 32;
-  const int lane = lane_id();
-  const T* q = static_cast<const T*>(p.q) + (s.q0 + token) * p.q_token + head * p.q_head;
-  float qf[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qf[e] = elem_to_float(q[lane * E + e]);
-    o[e] = 0.f;
+// The tiled product multiplies every value in a tile, and 0 * inf in a masked
+// place is a NaN in rows that do not see it.  A row whose sum is finite and whose
+// output is not is looked at again: attn_spoilt tells whether a key that it does
+// not see, among those of its masked steps, holds such a value, and only then
+// attn_row computes it over, without the keys that it does not see.  A value
+// that a row rightly sees costs the look alone (a NaN or infinity among its
+// scores not even that: its sum is NaN): one prompt of 8192 tokens whose first
+// value is NaN 620 us instead of 475.  Rows that are done over take 150 ns a key
+// with all eight warps at it (the same prompt with its last value NaN: 77 ms);
+// waits elsewhere in the CTA count from the last such row (WaitCtx::progress).
+
+// Whether a row of the request sees key j < m; bits: its mask.
+SVD_DEV bool attn_sees(const AttnParams& p, const AttnSeq& s, int token, unsigned long long bits, int j) {
+  if (!p.tree) return !p.causal || j <= s.first + token;
+  const int node = j - s.first;
+  return node < 0 || (p.mask != nullptr ? node < 64 && (bits >> node & 1) != 0 : node <= token);
+}
+
+// Where key j lies in k and v, in elements; false where its block is not in the cache.
+SVD_DEV bool attn_place(const AttnParams& p, const AttnSeq& s, int b, int kv_head, int j, int d, long long* k_at, long long* v_at) {
+  if (p.lens != nullptr) {
+    const int page = p.table[b * p.ld_table + (j >> p.block_shift)];
+    if (page < 0 || page >= p.num_blocks) return false;
+    const long long in = (kv_head * static_cast<long long>(p.block_size) + (j & (p.block_size - 1))) * d;
+    *k_at = page * p.k_token + in;
+    *v_at = page * p.v_token + in;
+  } else {
+    *k_at = (s.k0 + j) * p.k_token + kv_head * p.k_head;
+    *v_at = (s.k0 + j) * p.v_token + kv_head * p.v_head;
   }
-  const int sees = min(j_hi, p.causal ? s.first + token + 1 : s.m);
+  return true;
+}
+
+// Whether a key of [j_lo, j_hi) that this lane's row does not see has a value
+// that is not finite.  Called by whole warps of a tile that begins at token t0: a
+// lane reads a key, then each asks for its own row.
+template <typename T, int D>
+__device__ __forceinline__ bool attn_spoilt(const AttnParams& p, const AttnSeq& s, int b, int t0, int token, bool row_ok,
+                                         int kv_head, int j_lo, int j_hi) {
+  const int lane = static_cast<int>(lane_id());
+  const unsigned long long bits = p.mask != nullptr && row_ok ? p.mask[s.q0 + token] : 0;
+  j_lo = max(j_lo, p.tree ? s.first : p.causal ? s.first + t0 + 1 : s.m);  // every row of the tile sees the keys before
+  bool spoilt = false;
+  for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
+    float probe = 0.f;  // NaN when any element is not finite
+    long long k_at = 0, v_at = 0;
+    if (j0 + lane < j_hi && attn_place(p, s, b, kv_head, j0 + lane, D, &k_at, &v_at)) {
+      const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + v_at);
+#pragma unroll 8
+      for (int x = 0; x < D / 8; ++x) {
+        const uint4 w = v[x];
+        const float2 e[4] = {unpack_pair<T>(w.x), unpack_pair<T>(w.y), unpack_pair<T>(w.z), unpack_pair<T>(w.w)};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) probe = fmaf(e[y].x, 0.f, fmaf(e[y].y, 0.f, probe));
+      }
+    }
+    for (unsigned bad = __ballot_sync(0xffffffffu, probe != 0.f); bad != 0; bad &= bad - 1)
+      spoilt = spoilt || !attn_sees(p, s, token, bits, j0 + __ffs(bad) - 1);
+  }
+  return spoilt;
+}
+
+// The output of one row over the keys of [j_lo, j_hi) that it sees, a warp per
+// row, 32 keys at a time: a lane takes a key's product with q, then every lane
+// its elements of all 32 values.  `base` is the row's maximum, in the exponent's
+// units.
+template <typename T, int D>
+__device__ __forceinline__ void attn_row(const AttnParams& p, const AttnSeq& s, int b, int token, int head, int kv_head,
+                                      int j_lo, int j_hi, float base, float (&out)[D / 32]) {
+  constexpr int E = D / 32;
+  const int lane = static_cast<int>(lane_id());
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (s.q0 + token) * p.q_token + head * p.q_head);
+  float o[E] = {};  // not `out`: loads would wait for the stores to it
   const unsigned long long bits = p.mask != nullptr ? p.mask[s.q0 + token] : 0;
   const float c = p.neg ? -p.c : p.c;
-  for (int j = j_lo; j < sees; ++j) {
-    const T *kr, *vr;
-    if (p.lens != nullptr) {
-      const int node = j - s.first;
-      if (node >= 0 && (p.mask != nullptr ? node >= 64 || !(bits >> node & 1) : node > token)) continue;
-      const int page = p.table[b * p.ld_table + (j >> p.block_shift)];
-      if (page < 0 || page >= p.num_blocks) continue;
-      const long long in = (kv_head * static_cast<long long>(p.block_size) + (j & (p.block_size - 1))) * D;
-      kr = static_cast<const T*>(p.k) + page * p.k_token + in;
-      vr = static_cast<const T*>(p.v) + page * p.v_token + in;
-    } else {
-      kr = static_cast<const T*>(p.k) + (s.k0 + j) * p.k_token + kv_head * p.k_head;
-      vr = static_cast<const T*>(p.v) + (s.k0 + j) * p.v_token + kv_head * p.v_head;
+  for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
+    const int j = j0 + lane;
+    long long k_at = 0, v_at = 0;
+    const bool seen = j < j_hi && attn_sees(p, s, token, bits, j) && attn_place(p, s, b, kv_head, j, D, &k_at, &v_at);
+    float w = 0.f;
+    if (seen) {
+      const uint4* k = reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + k_at);
+      float2 dot = make_float2(0.f, 0.f);
+#pragma unroll 8
+      for (int x = 0; x < D / 8; ++x) {
+        const uint4 a = q[x], y = k[x];
+        dot = fma2(unpack_pair<T>(a.x), unpack_pair<T>(y.x), dot);
+        dot = fma2(unpack_pair<T>(a.y), unpack_pair<T>(y.y), dot);
+        dot = fma2(unpack_pair<T>(a.z), unpack_pair<T>(y.z), dot);
+        dot = fma2(unpack_pair<T>(a.w), unpack_pair<T>(y.w), dot);
+      }
+      w = exp2f((dot.x + dot.y) * c - base);
     }
-    float dot = 0.f;
+    const unsigned all = __ballot_sync(0xffffffffu, seen);
+    if (all == 0) continue;
+    // keys left out are read at another's place: no branch, so that the loads are in flight together
+    const long long other = __shfl_sync(0xffffffffu, v_at, __ffs(all) - 1);
+    if (!seen) v_at = other;
+#pragma unroll 16
+    for (int x = 0; x < 32; ++x) {
+      const float weight = __shfl_sync(0xffffffffu, w, x);
+      const T* v = static_cast<const T*>(p.v) + __shfl_sync(0xffffffffu, v_at, x) + lane * E;
+      const bool one = (all >> x & 1) != 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dot += qf[e] * elem_to_float(kr[lane * E + e]);
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float w = exp2f(dot * c - base);
+      for (int e = 0; e < E; e += 2) {
+        const float2 f = unpack_pair<T>(*reinterpret_cast<const uint32_t*>(v + e));
+        o[e] = one ? fmaf(weight, f.x, o[e]) : o[e];
+        o[e + 1] = one ? fmaf(weight, f.y, o[e + 1]) : o[e + 1];
+      }
+    }
+  }
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += w * elem_to_float(vr[lane * E + e]);
+  for (int e = 0; e < E; ++e) out[e] = o[e];
+}
+
+// The rows of a warp whose output is not finite, over again where a masked place
+// has reached them: written where the tiled result was, to the output (whole) or
+// to the worker's partial.  Every lane calls it with its own row.
+template <typename T, int D, bool PAIR>
+__device__ __noinline__ void attn_again(const AttnParams& p, const AttnSeq s, int b, int t0, int token, int head, int kv_head,
+                                        int row, bool odd, int j_lo, int j_hi, float base, float inv, float* part,
+                                        volatile unsigned long long* progress) {
+  constexpr int PART_ROWS = AttnCfg<D, PAIR>::PART_ROWS;
+  const int lane = static_cast<int>(lane_id());
+  unsigned redo = __ballot_sync(0xffffffffu, attn_spoilt<T, D>(p, s, b, t0, token, odd, kv_head, j_lo, j_hi) && odd);
+  while (redo != 0) {
+    const int src = __ffs(redo) - 1;
+    redo &= redo - 1;
+    const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
+    const int rw = __shfl_sync(0xffffffffu, row, src);
+    const float bs = __shfl_sync(0xffffffffu, base, src), iv = __shfl_sync(0xffffffffu, inv, src);
+    float o[D / 32];
+    attn_row<T, D>(p, s, b, tk, hd, kv_head, j_lo, j_hi, bs, o);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const int d = lane * (D / 32) + e;
+      if (part == nullptr)
+        static_cast<T*>(p.out)[static_cast<long long>(s.q0 + tk) * p.out_token + hd * p.out_head + d] =
+            elem_from_float<T>(o[e] * iv);
+      else
+        __stcg(part + (PAIR ? (d / 4 * PART_ROWS + rw) * 4 + d % 4 : rw * D + d), o[e]);
+    }
+    if (lane == 0) *progress = global_timer_ns();
   }
 }
 
@@ -455,6 +558,7 @@ struct AttnShared {
   uint32_t score_info[2][2];             // ... and the MMA warp hands on with the scores
   uint32_t tmem;
   int abort_flag;
+  unsigned long long progress;           // when a row was last done over
   AttnCut cut[3];
   long long per;
   long long scan[12];
@@ -750,6 +854,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&sh->kv_empty[i], Cfg::USERS);
     }
     sh->abort_flag = 0;
+    sh->progress = 0;
     fence_mbarrier_init();
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_k);
@@ -766,7 +871,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem;
-  const WaitCtx ctx{&sh->abort_flag, p.err, p.timeout_ns};
+  const WaitCtx ctx{&sh->abort_flag, p.err, p.timeout_ns, &sh->progress};
   // softmax group, MMA warp (8, 10) and TMA warp (9, 11) of worker wk
   const int wk = PAIR ? 0 : warp >= 8 ? (warp - 8) >> 1 : warp >> 2;
   Walk w;
@@ -1203,27 +1308,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           __stcg(part + Cfg::PART_ROWS * D + row, m == -INFINITY ? -INFINITY : base);
           __stcg(part + Cfg::PART_ROWS * (D + 1) + row, l);
         }
-        // rows that a masked place may have reached: over again, key by key
-        unsigned redo = __ballot_sync(0xffffffffu, row_ok && probe != 0.f);
-        while (redo != 0) {
-          const int src = __ffs(redo) - 1;
-          redo &= redo - 1;
-          const int tk = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
-          const int rw = __shfl_sync(0xffffffffu, row, src);
-          const float bs = __shfl_sync(0xffffffffu, base, src), iv = __shfl_sync(0xffffffffu, inv, src);
-          float o[D / 32];
-          attn_row<T, D>(p, w.s, w.b, tk, hd, kv_head, w.j0 * STEP, min(w.j1 * STEP, w.s.m), bs, o);
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) {
-            const int d = lane * (D / 32) + e;
-            if (whole)
-              static_cast<T*>(p.out)[static_cast<long long>(w.s.q0 + tk) * p.out_token + hd * p.out_head + d] =
-                  elem_from_float<T>(o[e] * iv);
-            else
-              __stcg(part + (PAIR ? (d / 4 * Cfg::PART_ROWS + rw) * 4 + d % 4 : rw * D + d), o[e]);
-          }
-        }
+        // rows that a masked place may have reached (a sum that is not finite: rightly so)
+        const bool odd = row_ok && probe != 0.f && l == l;
+        if (__any_sync(0xffffffffu, odd))
+          attn_again<T, D, PAIR>(p, w.s, w.b, t0, token, head, kv_head, row, odd, w.j0 * STEP, min(w.j1 * STEP, w.s.m), base,
+                                 inv, whole ? nullptr : part, &sh->progress);
       }
       tc_fence_before();
       if (!whole && w.j0 == 0) {                      // the worker's last segment: others go on with the unit

@@ -70,12 +70,14 @@ struct WaitCtx {
   volatile int* abort_flag;
   int* err;
   uint64_t limit_ns;
+  const volatile unsigned long long* progress = nullptr;  // when work that may take longer last got on (timer, ns)
 };
 
 // Waits until the phase with `parity` of `bar` completes.  Returns false if
-// the CTA was aborted or the wait exceeded ctx.limit_ns (then `site` is
-// recorded in the error word).  When `honour_abort` is false the wait ignores
-// the abort flag (used while draining copies that are still in flight).
+// the CTA was aborted or the wait exceeded ctx.limit_ns, counted from the last
+// progress (then `site` is recorded in the error word).  When `honour_abort` is
+// false the wait ignores the abort flag (used while draining copies that are
+// still in flight).
 SVD_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, int site,
                        bool honour_abort = true) {
   if (mbar_test(bar, parity)) return true;
@@ -84,7 +86,9 @@ SVD_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, int s
     if (mbar_test(bar, parity)) return true;
     if ((i & 31u) == 0u) {
       if (honour_abort && *ctx.abort_flag) return false;
-      if (global_timer_ns() - t0 > ctx.limit_ns) {
+      if (global_timer_ns() - t0 > ctx.limit_ns &&
+          (ctx.progress == nullptr ||
+           static_cast<int64_t>(global_timer_ns() - *ctx.progress) > static_cast<int64_t>(ctx.limit_ns))) {
         *ctx.abort_flag = 1;
         atomicCAS(ctx.err, 0, site);
         return false;
