@@ -591,7 +591,9 @@ int svdmlp_rope(const svdmlp_rope_args* args, void* stream);
  * left of the free list, *missing the blocks that it lacked (their entries and
  * slots are -1).  Tokens beyond a request's table_width * block_size places get
  * slot -1 too: lens tells them, *missing does not count them.  Only new table
- * entries are written: the call may be repeated.  Negative lengths count as 0.  No output overlaps an input. */
+ * entries are written: the call may be repeated.  Negative lengths count as 0,
+ * a request ends at 2^31 - 1 tokens, and the sums stop there.  No output
+ * overlaps an input. */
 typedef struct svdmlp_pages_args {
   int32_t batch, tokens, block_size, table_width, free_capacity, reserved;
   int32_t* table; /* [batch, ld_table] */

@@ -228,13 +228,38 @@ constexpr int kPagesChunk = 1024;  // requests scanned at a time
 // tokens of the chunk are then spread over all threads of the grid, each one
 // finding its request by bisection; CTA 0 writes what there is one of per
 // request.  A token in a new block takes the block's number from the free list
-// itself, so no CTA waits for another's table entries.  Latency-bound: one
-// scan and one bisection stand between the loads and the stores; 2.5 us for 8
-// requests of one token, 4.0 us for 1024 with up to 300 each (in a CUDA graph).
+// itself, so no CTA waits for another's table entries.  Lengths are not trusted:
+// a request ends at 2^31 - 1 tokens, and the sums stop there, so that no place
+// is ever worked out of a wrapped one; a chunk with a length of kPagesCalm or more is
+// added up one by one.  Latency-bound: one scan and one bisection stand between
+// the loads and the stores; 2.5 us for 8 requests of one token, 4.1 us for 1024
+// with up to 300 each (in a CUDA graph).
+
+constexpr int kPagesCalm = 1 << 21;  // lengths and widths below it have sums below 2^31 over a chunk
+
+// a + b for a, b >= 0, at most 2^31 - 1.
+SVD_DEV int capped_sum(int a, int b) { return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), 0x7fffffffu)); }
+
+// Tokens held and added of one request, and the blocks that it has and lacks.
+struct PagesRequest {
+  int held, added, have, lacks;
+};
+SVD_DEV PagesRequest load_request(const PagesParams& p, int b) {
+  PagesRequest r{0, 0, 0, 0};
+  if (b < p.batch) {
+    r.held = max(p.held[b], 0);
+    r.added = min(max(p.added[b], 0), 0x7fffffff - r.held);
+  }
+  const unsigned size = p.block_size, up = size - 1;
+  r.have = static_cast<int>(min((r.held + up) / size, static_cast<unsigned>(p.width)));
+  r.lacks = static_cast<int>(min((r.held + r.added + up) / size, static_cast<unsigned>(p.width))) - r.have;
+  return r;
+}
+
 __global__ void __launch_bounds__(kPagesThreads) page_step_kernel(const PagesParams p) {
   constexpr int PER = kPagesChunk / kPagesThreads;
   __shared__ int s_cu[kPagesChunk + 1];    // first new token of each request of the chunk
-  __shared__ int s_take[kPagesChunk];      // blocks taken before it
+  __shared__ int s_take[kPagesChunk + 1];  // blocks taken before it
   __shared__ int s_held[kPagesChunk];
   __shared__ unsigned long long s_warp[kPagesThreads / 32];
   grid_dependency_wait();
@@ -242,29 +267,26 @@ __global__ void __launch_bounds__(kPagesThreads) page_step_kernel(const PagesPar
   const int left = max(0, min(*p.free_count, p.capacity));
   int cu0 = 0, take0 = 0;  // carried over the chunks
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // places among the tokens and blocks of a chunk; unsigned, as a stride may go beyond 2^31
+  const unsigned first = blockIdx.x * kPagesThreads + threadIdx.x, stride = gridDim.x * kPagesThreads;
   const auto table_page = [&](int b, int have, int take, int idx) -> int {
     if (idx >= p.width) return -1;
     if (idx < have) return p.table[b * p.ld_table + idx];
-    const int at = take + idx - have;
+    const int at = capped_sum(take, idx - have);
     return at < left ? p.free_blocks[left - 1 - at] : -1;
   };
   for (int b0 = 0; b0 < p.batch; b0 += kPagesChunk) {
     // running sums, (blocks << 32 | tokens) in one word; each thread owns PER requests in a row
     unsigned long long mine[PER], sum = 0;
     int held[PER];
+    bool wild = p.width >= kPagesCalm;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int b = b0 + threadIdx.x * PER + i;
-      int h = 0, n = 0;
-      if (b < p.batch) {
-        h = max(p.held[b], 0);
-        n = max(p.added[b], 0);
-      }
-      held[i] = h;
-      const int have = min((h + p.block_size - 1) / p.block_size, p.width);
-      const int need = min((h + n + p.block_size - 1) / p.block_size, p.width);
+      const PagesRequest r = load_request(p, b0 + threadIdx.x * PER + i);
+      wild = wild || r.added >= kPagesCalm;
+      held[i] = r.held;
       mine[i] = sum;
-      sum += static_cast<unsigned long long>(need - have) << 32 | static_cast<unsigned>(n);
+      sum += static_cast<unsigned long long>(r.lacks) << 32 | static_cast<unsigned>(r.added);
     }
     unsigned long long inc = sum;
 #pragma unroll
@@ -273,55 +295,91 @@ __global__ void __launch_bounds__(kPagesThreads) page_step_kernel(const PagesPar
       if (lane >= o) inc += up;
     }
     if (lane == 31) s_warp[warp] = inc;
-    __syncthreads();
-    unsigned long long before = 0, all = 0;
+    int cu1 = 0, take1 = 0;
+    const bool calm = __syncthreads_or(wild) == 0;
+    if (calm) {
+      unsigned long long before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPagesThreads / 32; ++w) {
-      if (w < warp) before += s_warp[w];
-      all += s_warp[w];
-    }
-    before += inc - sum;
+      for (int w = 0; w < kPagesThreads / 32; ++w) {
+        if (w < warp) before += s_warp[w];
+        all += s_warp[w];
+      }
+      before += inc - sum;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const unsigned long long at = before + mine[i];
-      s_cu[threadIdx.x * PER + i] = cu0 + static_cast<int>(at & 0xffffffffu);
-      s_take[threadIdx.x * PER + i] = take0 + static_cast<int>(at >> 32);
-      s_held[threadIdx.x * PER + i] = held[i];
+      for (int i = 0; i < PER; ++i) {
+        const unsigned long long at = before + mine[i];
+        s_cu[threadIdx.x * PER + i] = capped_sum(cu0, static_cast<int>(at & 0xffffffffu));
+        s_take[threadIdx.x * PER + i] = capped_sum(take0, static_cast<int>(at >> 32));
+        s_held[threadIdx.x * PER + i] = held[i];
+      }
+      cu1 = capped_sum(cu0, static_cast<int>(all & 0xffffffffu));
+      take1 = capped_sum(take0, static_cast<int>(all >> 32));
+      if (threadIdx.x == 0) s_cu[kPagesChunk] = cu1;
+    } else if (threadIdx.x == 0) {  // sums that the halves of a word may not hold: one after another
+      int cu = cu0, take = take0;
+      for (int i = 0; i < kPagesChunk; ++i) {
+        const PagesRequest r = load_request(p, b0 + i);
+        s_cu[i] = cu;
+        s_take[i] = take;
+        s_held[i] = r.held;
+        cu = capped_sum(cu, r.added);
+        take = capped_sum(take, r.lacks);
+      }
+      s_cu[kPagesChunk] = cu;
+      s_take[kPagesChunk] = take;
     }
-    const int cu1 = cu0 + static_cast<int>(all & 0xffffffffu), take1 = take0 + static_cast<int>(all >> 32);
-    if (threadIdx.x == 0) s_cu[kPagesChunk] = cu1;
     __syncthreads();
 
     const int here = min(kPagesChunk, p.batch - b0);
+    if (!calm) {
+      cu1 = s_cu[kPagesChunk];
+      take1 = s_take[kPagesChunk];
+    }
     if (blockIdx.x == 0) {
       for (int i = threadIdx.x; i < here; i += kPagesThreads) {
         p.cu[b0 + i] = s_cu[i];
-        p.lens[b0 + i] = s_held[i] + s_cu[i + 1] - s_cu[i];
+        p.lens[b0 + i] = s_held[i] + (s_cu[i + 1] - s_cu[i]);
       }
     }
-    for (int t = cu0 + blockIdx.x * kPagesThreads + threadIdx.x; t < cu1; t += gridDim.x * kPagesThreads) {
-      int lo = 0, hi = here;  // the last request that starts at or before t
+    // the last request of the chunk that begins at or before x
+    const auto request_of = [&](const int* begins, int x) -> int {
+      int lo = 0, hi = here;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= t) lo = mid;
+        if (begins[mid] <= x) lo = mid;
         else hi = mid;
       }
-      const int pos = s_held[lo] + t - s_cu[lo];
+      return lo;
+    };
+    const auto have_of = [&](int lo) -> int {
+      const unsigned size = p.block_size;
+      return static_cast<int>(min((s_held[lo] + (size - 1)) / size, static_cast<unsigned>(p.width)));
+    };
+    const unsigned end = cu1 > p.tokens ? p.tokens : cu1;
+    for (unsigned t = cu0 + first; t < end; t += stride) {
+      const int lo = request_of(s_cu, static_cast<int>(t));
+      const int pos = s_held[lo] + (static_cast<int>(t) - s_cu[lo]);
       const int idx = pos / p.block_size, off = pos - idx * p.block_size;
-      const int have = min((s_held[lo] + p.block_size - 1) / p.block_size, p.width);
-      const int page = table_page(b0 + lo, have, s_take[lo], idx);
-      if (t < p.tokens) {
+      const int have = have_of(lo), page = table_page(b0 + lo, have, s_take[lo], idx);
+      if (t < static_cast<unsigned>(p.tokens)) {  // always; without the question the loads come later (2.71 for 2.53 us)
         p.slots[t] = page >= 0 ? static_cast<long long>(page) * p.block_size + off : -1;
         p.positions[t] = pos;
       }
       // the first token of a new block enters it into the table
       if (idx >= have && idx < p.width && off == 0) p.table[(b0 + lo) * p.ld_table + idx] = page;
     }
+    if (cu1 > p.tokens) {  // more tokens than the caller said: their blocks by themselves
+      for (unsigned x = take0 + first; x < static_cast<unsigned>(take1); x += stride) {
+        const int lo = request_of(s_take, static_cast<int>(x));
+        const int have = have_of(lo), idx = have + (static_cast<int>(x) - s_take[lo]);
+        if (idx < p.width) p.table[(b0 + lo) * p.ld_table + idx] = table_page(b0 + lo, have, s_take[lo], idx);
+      }
+    }
     cu0 = cu1;
     take0 = take1;
     __syncthreads();
   }
-  for (int t = cu0 + blockIdx.x * kPagesThreads + threadIdx.x; t < p.tokens; t += gridDim.x * kPagesThreads) {
+  for (unsigned t = cu0 + first; t < static_cast<unsigned>(p.tokens); t += stride) {
     p.slots[t] = -1;
     p.positions[t] = 0;
   }

@@ -427,7 +427,8 @@ def page_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     free_count.  `missing` above zero means that the free list ran out: those
     blocks' entries and slots are -1.  A request's tokens beyond the table's
     W * block_size places get slot -1 too; they count in seq_lens, which tells
-    them, and not in `missing`."""
+    them, and not in `missing`.  Negative lengths count as 0, and a request ends
+    at 2^31 - 1 tokens."""
     try:
         b, width = block_table.shape
         index, one = block_table.get_device(), (1,)
