@@ -60,6 +60,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "attention_line.h"
 #include "rope_pages.cuh"
 
 namespace svdmlp {
@@ -667,11 +668,11 @@ SVD_DEV void find_cuts(const AttnParams& p, AttnShared* sh) {
     if (lane == 0) {
       const int in = static_cast<int>(rem - steps_before<STEP>(p, s, w, lo) - static_cast<long long>(lo) * kUnitCost<PAIR>);
       const int steps = tile_steps<STEP>(p, s, w, lo);
-      int j = in - kUnitCost<PAIR>;
-      if (j <= 0 || steps <= p.snap) {  // at the unit's start, or the next one's where that is nearer
-        j = 0;
+      int j = cut_step(in, steps, kUnitCost<PAIR>, p.snap);
+      if (j == 0 || j == steps) {  // at the unit's start, or the next one's
         at -= in;
-        if (2 * in > steps + kUnitCost<PAIR>) {
+        if (j == steps) {
+          j = 0;
           at += steps + kUnitCost<PAIR>;
           if (++lo == tiles_of(s, w)) {
             lo = 0;

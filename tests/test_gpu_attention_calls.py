@@ -59,3 +59,16 @@ def test_tree_out_apart_from_the_cache(cuda_device, att):
     wide = torch.zeros(3, 2, d, dtype=BF16, device="cuda")
     att.tree_attention(q, k, v, *args, max_tree=1, out=wide[1:2])
     assert torch.equal(wide[1:2], want) and not wide[0].any() and not wide[2].any()
+
+
+@pytest.mark.parametrize("batch,width", [(1, 3), (3, 3), (9, 20), (30, 3)])
+def test_units_just_longer_than_those_left_whole(cuda_device, att, batch, width):
+    """Three steps a unit, with few and with many units: cuts everywhere in them."""
+    news, lens = [33 + i % 32 for i in range(batch)], [257 + (i * 37) % 128 for i in range(batch)]
+    k, v, table = _paged(11, lens, 2, 64, 128, BF16)
+    table = torch.nn.functional.pad(table, (0, max(0, width - table.shape[1])), value=-1).contiguous()
+    q = _randn(12, sum(news), 8, 64)
+    args = table, torch.tensor(lens, dtype=torch.int32, device="cuda"), ref.cumulative(news, cuda_device)
+    outs = [att.tree_attention(q, k, v, *args, max_tree=64) for _ in range(3)]
+    ref.check(outs[0], *ref.tree(q, k, v, table, lens, news, None), BF16, f"{batch}")
+    assert all(torch.equal(o, outs[0]) for o in outs)
