@@ -162,6 +162,11 @@ int svdmlp_workspace_init(void* workspace, int64_t workspace_bytes, void* stream
  * control block re-armed), so the next call reports only later launches. */
 int svdmlp_check_device_status(void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The id of the CUDA graph capture that `stream` is in, 0 outside one.  A
+ * workspace that a capture has used belongs to the graph: it must outlive it, and
+ * no other call may use it while the graph runs. */
+int svdmlp_stream_capture_id(void* stream, uint64_t* id);
+
 /* ---------------------------------------------------------------- operators */
 /*
  * Fused low-rank gate/up operator: h[M, ff] = SiLU(x.u_gate.v_gate) * (x.u_up.v_up).

@@ -1706,6 +1706,15 @@ static int read_error_block(const void* block, cudaStream_t s, int* status) {
   return SVDMLP_OK;
 }
 
+int svdmlp_stream_capture_id(void* stream, uint64_t* id) {
+  if (!id) return SVDMLP_ERR_INVALID_VALUE;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long found = 0;
+  SVD_CUDA(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &found));
+  *id = status == cudaStreamCaptureStatusNone ? 0 : found;
+  return SVDMLP_OK;
+}
+
 int svdmlp_check_device_status(void* ws, int64_t ws_bytes, void* stream) {
   if (!ws || ws_bytes < kCtlBytes) return SVDMLP_ERR_INVALID_VALUE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

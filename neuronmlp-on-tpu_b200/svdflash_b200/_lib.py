@@ -102,6 +102,7 @@ SIGNATURES = {
     "svdmlp_workspace_bytes": (c_int64, [LP, c_int]),
     "svdmlp_workspace_init": (c_int, [V, I64, V]),
     "svdmlp_check_device_status": (c_int, [V, I64, V]),
+    "svdmlp_stream_capture_id": (c_int, [V, V]),
     "svdmlp_pack_status": (c_int, [LP, V, V]),
     "svdmlp_gate_up": (c_int, [LP, V, V, I64, c_int, V, I64, V, I64, V]),
     "svdmlp_xuv": (c_int, [LP, V, V, I64, c_int, V, I64, V, I64, V]),

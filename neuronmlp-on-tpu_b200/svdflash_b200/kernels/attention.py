@@ -43,6 +43,7 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 # checks have to as well); only where that fails, _refuse_* name what is wrong.
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch.cuda.current_device
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 _PLAIN = torch.contiguous_format
 _MASK_BITS = 64  # tree tokens that a row's mask names
 
@@ -228,9 +229,10 @@ def _workspace(device: torch.device, head_dim: int):
         with torch.cuda.device(device):
             need = max(int(lib.svdmlp_prompt_workspace_bytes()), int(lib.svdmlp_tree_workspace_bytes(head_dim)))
         _workspace_need[device.index, head_dim] = need
-    with ops._ws_lock:
-        ws = ops._ws_pool.get((device.index, _stream(device.index)))
-    if ws is not None and ws.nbytes >= need:
+    # the usual case without a lock: reading the pool is one step
+    index = device.index
+    ws = ops._ws_pool.get((index, _stream(index)))
+    if ws is not None and ws.nbytes >= need and index == _device() and not _capturing():
         return ws
     return ops.workspace_for(device, need)
 

@@ -120,30 +120,73 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 # ----------------------------------------------------------------- workspace
 _ws_lock = threading.Lock()
-_ws_pool: dict = {}
+_ws_pool: dict = {}       # (device index, stream): the workspace of calls there
+_ws_kept: list = []       # (key, workspace): replaced ones that a CUDA graph writes at every replay
+_ws_captures: dict = {}   # (device index, stream): one that the latest capture there made for itself
 
 
 class _Workspace:
-    def __init__(self, device: torch.device, nbytes: int):
-        self.tensor = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    """`capture`: the id of the capture that makes it (0: none).  Then its
+    memory is the graph's own and is set up by the graph, at every replay."""
+
+    def __init__(self, device: torch.device, nbytes: int, capture: int = 0):
         self.nbytes = int(nbytes)
+        self.capture = capture
+        self.captured = False     # used by a capture: a graph goes on writing it
+        self.tensor = torch.empty(self.nbytes + (_READY if capture else 0), dtype=torch.uint8, device=device)
         _lib.check(_lib.load().svdmlp_workspace_init(self.ptr, self.nbytes, _stream(device)), "workspace_init")
+        if capture:
+            self.tensor[self.nbytes:].fill_(_READY_BYTE)
 
     @property
     def ptr(self) -> int:
         return self.tensor.data_ptr()
 
+    def ready(self) -> bool:
+        """Whether it has been set up (one of a graph: whether that has run)."""
+        return not self.capture or bool((self.tensor[self.nbytes:] == _READY_BYTE).all())
+
+
+_READY, _READY_BYTE = 64, 0xA7   # bytes behind a graph's workspace that its replays fill
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _capture_id(index: int, stream: int) -> int:
+    """The id of the capture that `stream`, the device's current one, is in; 0 outside one."""
+    if index == torch.cuda.current_device() and not torch.cuda.is_current_stream_capturing():
+        return 0
+    found = ctypes.c_uint64()
+    _lib.check(_lib.load().svdmlp_stream_capture_id(ctypes.c_void_p(stream), ctypes.byref(found)), "stream_capture_id")
+    return found.value
+
 
 def workspace_for(device: torch.device, nbytes: int) -> _Workspace:
-    """Per-(device, stream) workspace, grown on demand and then reused."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    """Per-(device, stream) workspace, grown on demand and then reused.
+
+    A workspace that a capture has used stays alive when a larger one replaces
+    it.  A capture that needs more than the stream has gets one of its own: it
+    cannot wait for the stream."""
+    key = index, stream = device.index, _raw_stream(device.index)
+    capture = _capture_id(index, stream)
     with _ws_lock:
         ws = _ws_pool.get(key)
-        if ws is None or ws.nbytes < nbytes:
-            if ws is not None:
-                torch.cuda.current_stream(device).synchronize()
-            ws = _Workspace(device, max(int(nbytes), 1 << 20))
-            _ws_pool[key] = ws
+        if ws is not None and ws.nbytes >= nbytes:
+            if capture:
+                ws.captured = True
+            return ws
+        size = max(int(nbytes), 1 << 20)
+        if capture:
+            ws = _ws_captures.get(key)
+            if ws is None or ws.capture != capture or ws.nbytes < nbytes:
+                ws = _ws_captures[key] = _Workspace(device, size, capture)
+            return ws
+        if ws is not None:
+            torch.cuda.current_stream(device).synchronize()
+            if ws.captured:
+                _ws_kept.append((key, ws))
+        ws = _ws_pool[key] = _Workspace(device, size)
     return ws
 
 
@@ -153,9 +196,9 @@ def check_device_status(device: Optional[torch.device] = None) -> None:
     since the last check."""
     lib = _lib.load()
     with _ws_lock:
-        items = list(_ws_pool.items())
+        items = [*_ws_pool.items(), *_ws_kept, *_ws_captures.items()]
     for (dev_index, stream), ws in items:
-        if device is not None and device.index != dev_index:
+        if (device is not None and device.index != dev_index) or not ws.ready():
             continue
         _lib.check(lib.svdmlp_check_device_status(ws.ptr, ws.nbytes, ctypes.c_void_p(stream)), "device status")
 
