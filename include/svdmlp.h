@@ -152,7 +152,9 @@ int svdmlp_dense_pack(const svdmlp_layout* layout, const void* w_gate, int64_t l
 int64_t svdmlp_workspace_bytes(const svdmlp_layout* layout, int max_m);
 
 /* Zeroes the workspace control block (error word and split-K counters).
- * Call once after allocating a workspace; the kernels keep it clean after. */
+ * Call once after allocating a workspace; the kernels keep it clean after.  An
+ * entry point's launches meet in the workspace: calls on it follow one another,
+ * on one stream and from one thread at a time. */
 int svdmlp_workspace_init(void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Synchronises `stream`, then reports SVDMLP_ERR_DEVICE_TIMEOUT if a device

@@ -24,6 +24,7 @@ is for inference).
 from __future__ import annotations
 
 import math
+import threading
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -42,7 +43,8 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 # comparisons (a decoding step's launches take a few microseconds each, so the
 # checks have to as well); only where that fails, _refuse_* name what is wrong.
 _stream = torch._C._cuda_getCurrentRawStream
-_device = torch.cuda.current_device
+_device = torch._C._cuda_getDevice
+_thread = threading.get_ident
 _capturing = torch._C._cuda_isCurrentStreamCapturing
 _PLAIN = torch.contiguous_format
 _MASK_BITS = 64  # tree tokens that a row's mask names
@@ -222,7 +224,7 @@ _workspace_need: dict = {}
 
 
 def _workspace(device: torch.device, head_dim: int):
-    """The attention workspace of the device's current stream: the pool that the other operators use."""
+    """The attention workspace of the device's current stream and this thread: the pool that the other operators use."""
     need = _workspace_need.get((device.index, head_dim))
     if need is None:
         lib = _lib.load()
@@ -231,7 +233,7 @@ def _workspace(device: torch.device, head_dim: int):
         _workspace_need[device.index, head_dim] = need
     # the usual case without a lock: reading the pool is one step
     index = device.index
-    ws = ops._ws_pool.get((index, _stream(index)))
+    ws = ops._ws_pool.get((index, _stream(index), _thread()))
     if ws is not None and ws.nbytes >= need and index == _device() and not _capturing():
         return ws
     return ops.workspace_for(device, need)

@@ -120,9 +120,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 # ----------------------------------------------------------------- workspace
 _ws_lock = threading.Lock()
-_ws_pool: dict = {}       # (device index, stream): the workspace of calls there
+_ws_pool: dict = {}       # (device index, stream, thread): the workspace of calls there
 _ws_kept: list = []       # (key, workspace): replaced ones that a CUDA graph writes at every replay
-_ws_captures: dict = {}   # (device index, stream): one that the latest capture there made for itself
+_ws_captures: dict = {}   # as _ws_pool: one that the latest capture there made for itself
 
 
 class _Workspace:
@@ -162,16 +162,33 @@ def _capture_id(index: int, stream: int) -> int:
     return found.value
 
 
-def workspace_for(device: torch.device, nbytes: int) -> _Workspace:
-    """Per-(device, stream) workspace, grown on demand and then reused.
+def _take_over(key):
+    """The workspace that a thread which has ended left on key's stream, now key's; or None."""
+    threading.current_thread()     # from here on in enumerate(), whoever started it
+    alive = {t.ident for t in threading.enumerate()}
+    for other in _ws_pool:
+        if other[:2] == key[:2] and other[2] not in alive:
+            ws = _ws_pool[key] = _ws_pool.pop(other)
+            return ws
+    return None
 
-    A workspace that a capture has used stays alive when a larger one replaces
-    it.  A capture that needs more than the stream has gets one of its own: it
-    cannot wait for the stream."""
-    key = index, stream = device.index, _raw_stream(device.index)
+
+def workspace_for(device: torch.device, nbytes: int) -> _Workspace:
+    """Workspace of this stream and thread, grown on demand and then reused.
+
+    A call is several launches that meet in the workspace, and another thread's
+    may come between them on the same stream: each thread has its own, and a new
+    one takes over what a thread that has ended left on the stream.  A workspace
+    that a capture has used stays alive when a larger one replaces it.  A capture
+    that needs more than there is gets one of its own: it cannot wait for the
+    stream."""
+    index, stream = device.index, _raw_stream(device.index)
+    key = index, stream, threading.get_ident()
     capture = _capture_id(index, stream)
     with _ws_lock:
         ws = _ws_pool.get(key)
+        if ws is None:
+            ws = _take_over(key)
         if ws is not None and ws.nbytes >= nbytes:
             if capture:
                 ws.captured = True
@@ -197,7 +214,7 @@ def check_device_status(device: Optional[torch.device] = None) -> None:
     lib = _lib.load()
     with _ws_lock:
         items = [*_ws_pool.items(), *_ws_kept, *_ws_captures.items()]
-    for (dev_index, stream), ws in items:
+    for (dev_index, stream, _), ws in items:
         if (device is not None and device.index != dev_index) or not ws.ready():
             continue
         _lib.check(lib.svdmlp_check_device_status(ws.ptr, ws.nbytes, ctypes.c_void_p(stream)), "device status")

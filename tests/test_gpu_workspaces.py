@@ -2,6 +2,8 @@
 workspace."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -92,3 +94,30 @@ def test_a_decoding_step_captured_without_a_warm_stream(cuda_device, model):
     decs[0].check()
     assert decs[0].seq_lens.tolist() == decs[1].seq_lens.tolist() == [40]
     assert torch.equal(torch.cat(outs[1:]), torch.cat(want))
+
+
+def test_threads_on_one_stream(cuda_device, att):
+    """Divided units of two shapes from several threads at once: each thread's launches meet in its own workspace."""
+    from svdflash_b200.kernels import ops
+    calls, wants, wrong = [], [], []
+    for news, lens in ([[1], [9000]], [[20], [3000]], [[1, 1], [5000, 70]], [[40], [4000]]):
+        k, v, table = _paged(len(news) + lens[0], lens, 2, 128, 16, torch.bfloat16)
+        q = _randn(3, sum(news), 8, 128)
+        args = q, k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), ref.cumulative(news, cuda_device)
+        calls.append(lambda args=args, most=max(news): att.tree_attention(*args, max_tree=most))
+        wants.append(calls[-1]())
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(calls))
+
+    def work(call, want):
+        start.wait()
+        outs = [call() for _ in range(200)]
+        torch.cuda.synchronize()
+        wrong.append(sum(not torch.equal(o, want) for o in outs))
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(calls, wants)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0] * len(calls)
+    ops.check_device_status(cuda_device)

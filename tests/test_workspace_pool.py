@@ -1,6 +1,7 @@
 """The pool of workspaces, with workspaces that are only sizes: what is reused, replaced and kept."""
 from __future__ import annotations
 
+import threading
 import types
 
 import pytest
@@ -76,3 +77,48 @@ def test_a_capture_on_a_stream_without_one(pool):
     assert own.capture == 5 and pool.get(1000) is own and pool.ops._ws_pool == {}
     pool.capture = 0
     assert pool.get(10).capture == 0
+
+
+def _in_thread(call):
+    got = []
+    thread = threading.Thread(target=lambda: got.append(call()))
+    thread.start()
+    thread.join()
+    return got[0]
+
+
+def test_threads_on_one_stream_do_not_share(pool):
+    """A call's launches meet in its workspace, and another thread's launches may come between them."""
+    mine, meet = pool.get(100), threading.Barrier(3)
+    theirs = []
+
+    def work():
+        ws = pool.get(100)
+        theirs.append(ws)
+        meet.wait()
+        assert pool.get(100) is ws
+        meet.wait()
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    meet.wait()
+    assert pool.get(100) is mine
+    meet.wait()
+    for t in threads:
+        t.join()
+    assert len({id(ws) for ws in theirs + [mine]}) == 3
+
+
+def test_threads_that_have_ended_leave_theirs(pool):
+    """Short-lived threads do not pile workspaces up; one that is too small for its heir grows."""
+    mine = pool.get(100)
+    first = _in_thread(lambda: pool.get(1 << 21))
+    assert first is not mine
+    for _ in range(5):
+        assert _in_thread(lambda: pool.get(1 << 21)) is first
+    larger = _in_thread(lambda: pool.get(1 << 22))
+    assert larger is not first and pool.waits == 1
+    pool.stream = 8
+    assert _in_thread(lambda: pool.get(100)) is not larger     # of another stream
+    pool.stream = 7
+    assert pool.get(100) is mine and len(pool.ops._ws_pool) == 3
