@@ -254,8 +254,10 @@ def rope_frequencies(head_dim: int, *, base: float = 10000.0, rotary_dim: Option
       blend of the two between;
     * ``yarn``: the same between the pairs that turn ``beta_fast`` (32) and
       ``beta_slow`` (1) times over the original context, linear in the pair's
-      index, and a magnitude of 0.1 ln(factor) + 1 (``attention_factor``
-      overrides it).
+      index, from whole pairs unless ``truncate`` is false, and a magnitude of
+      0.1 ln(factor) + 1; with ``mscale`` and ``mscale_all_dim`` the quotient of
+      0.1 mscale ln(factor) + 1 and the same of mscale_all_dim;
+      ``attention_factor`` overrides both.
     """
     rot = head_dim if rotary_dim is None else rotary_dim
     if isinstance(rot, bool) or not isinstance(rot, int) or rot <= 0 or rot % 2 or rot > head_dim:
@@ -282,12 +284,25 @@ def rope_frequencies(head_dim: int, *, base: float = 10000.0, rotary_dim: Option
         def pair_that_turns(times):
             return half * math.log(context / (2 * math.pi * times)) / math.log(base)
 
-        first = max(math.floor(pair_that_turns(scaling.get("beta_fast", 32))), 0)
-        last = min(math.ceil(pair_that_turns(scaling.get("beta_slow", 1))), rot - 1)
+        def magnitude_of(times):
+            return 0.1 * times * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        first, last = pair_that_turns(scaling.get("beta_fast", 32)), pair_that_turns(scaling.get("beta_slow", 1))
+        if scaling.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rot - 1)
         span = max(last - first, 0.001)
         keep = [1 - min(1.0, max(0.0, (i - first) / span)) for i in range(half)]
         freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
-        magnitude = scaling.get("attention_factor") or (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        scales = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        if scaling.get("attention_factor"):
+            magnitude = scaling["attention_factor"]
+        elif all(scales):
+            magnitude = magnitude_of(scales[0]) / magnitude_of(scales[1])
+        elif scales[0] not in (None, 1) or scales[1] is not None:
+            raise ValueError("mscale and mscale_all_dim go together: one of them alone has no one meaning")
+        else:
+            magnitude = magnitude_of(1.0)
     elif kind != "default":
         raise ValueError(f"unknown rotary scaling {kind!r} (default, linear, llama3, yarn)")
     return torch.tensor(freq, dtype=torch.float32, device=device), float(magnitude)

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import math
 import random
 
 import pytest
@@ -51,3 +52,37 @@ def test_overlaps_of_usual_layouts_need_no_search(monkeypatch):
                  (heads_first[:, :4], heads_first[:, 4:]), (heads_first[:, ::2], heads_first[:, 1::2]),
                  (qkv, torch.zeros(300, 6, 8)), (blocks[:, :1], blocks[:, 1:])]:
         assert not attention._overlap(a, b)
+
+
+# --------------------------------------------------- yarn's magnitude and ends
+YARN = dict(type="yarn", factor=40.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("more,want", [
+    ({}, 0.1 * math.log(40) + 1), (dict(mscale=1.0), 0.1 * math.log(40) + 1), (dict(mscale=1.0, mscale_all_dim=1.0), 1.0),
+    (dict(mscale=0.707, mscale_all_dim=1.0), (0.0707 * math.log(40) + 1) / (0.1 * math.log(40) + 1)),
+    (dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.25), 1.25), (dict(mscale=1.0, mscale_all_dim=0.5, factor=1.0), 1.0)])
+def test_yarn_magnitude(more, want):
+    from svdflash_b200.kernels import attention as att
+    got = att.rope_frequencies(64, device="cpu", scaling={**YARN, **more})[1]
+    assert got == pytest.approx(want, rel=1e-12)
+
+
+@pytest.mark.parametrize("more", [dict(mscale=0.7), dict(mscale_all_dim=0.7), dict(mscale=0.7, mscale_all_dim=0), dict(mscale=0)])
+def test_half_of_yarns_magnitude_is_refused(more):
+    from svdflash_b200.kernels import attention as att
+    with pytest.raises(ValueError, match="mscale"):
+        att.rope_frequencies(64, device="cpu", scaling={**YARN, **more})
+
+
+def test_yarn_between_its_ends():
+    """The share of the stretched frequency grows evenly with the pair's index between the ends, whole pairs or not."""
+    from svdflash_b200.kernels import attention as att
+    half, base = 32, 10000.0
+    ends = [half * math.log(4096 / (2 * math.pi * turns)) / math.log(base) for turns in (32, 1)]
+    for more, (first, last) in (({}, (math.floor(ends[0]), math.ceil(ends[1]))), (dict(truncate=False), ends)):
+        freq, _ = att.rope_frequencies(64, base=base, device="cpu", scaling={**YARN, **more})
+        for i in range(half):
+            plain = base ** (-i / half)
+            share = min(1.0, max(0.0, (i - first) / (last - first)))
+            assert freq[i].item() == pytest.approx(plain * (1 - share) + plain / 40 * share, rel=1e-6)
