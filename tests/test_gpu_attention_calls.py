@@ -72,3 +72,14 @@ def test_units_just_longer_than_those_left_whole(cuda_device, att, batch, width)
     outs = [att.tree_attention(q, k, v, *args, max_tree=64) for _ in range(3)]
     ref.check(outs[0], *ref.tree(q, k, v, table, lens, news, None), BF16, f"{batch}")
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_a_chain_of_hundreds_behind_a_long_context(cuda_device, att):
+    """A prompt's next chunk over the cache."""
+    news, lens = [512, 300, 1], [4512, 9000, 700]
+    k, v, table = _paged(13, lens, 2, 128, 16, BF16)
+    q = _randn(14, sum(news), 8, 128)
+    args = table, torch.tensor(lens, dtype=torch.int32, device="cuda"), ref.cumulative(news, cuda_device)
+    want = ref.tree(q, k, v, table, lens, news, None)
+    for most in (512, 1):
+        ref.check(att.tree_attention(q, k, v, *args, max_tree=most), *want, BF16, f"max_tree {most}")
