@@ -41,7 +41,8 @@
 // the tensor pipe and on the exponential unit; P V starts on the first 64 keys
 // while the exponentials of the others are computed.  (With two tiles of 64 the
 // issue of the products bounds PAIR, with or without a softmax: 565 us where
-// this takes 490, at one prompt of 8192 tokens, 32 and 8 heads of 128.)  The
+// this took 490, a few calls at a time, at one prompt of 8192 tokens, 32 and 8
+// heads of 128.)  The
 // output is rescaled only when a row's maximum grows by more than 8 (in powers of
 // two): a stale base keeps probabilities below 2^8, which the 16-bit types and
 // the fp32 sums hold without loss.
@@ -50,8 +51,10 @@
 // tensor pipe takes 1100 cycles and the exponential unit 1024, and the chain
 // scores -> maximum -> exponentials -> P V -> scores of a tile some 3000, so that
 // two tiles in turn leave gaps in both (without the softmax's arithmetic the
-// same products take 395 instead of 490 us); in calls that follow one another
-// for long the power limit takes the clock down, to 540 us.  Few rows on many
+// same products took 395 instead of 490 us); 513 us for a call after a pause over
+// other inputs, 545 to 565 in calls that follow one another for long, where the
+// power limit takes the clock down.  The PAIR kernels spill some 300 bytes a
+// thread around the softmax (168 registers at launch).  Few rows on many
 // keys: the bytes of k and v, read once; for short calls the start of the CTAs
 // (the cuts 2 to 4 us, block tables and first loads 3) and the join.  One token on
 // 65537 keys: 54 us, 5.1 TB/s, and 5 us for the join.
@@ -572,7 +575,7 @@ constexpr uint32_t kInfoFirst = 4, kInfoLast = 8; // first, last step of the seg
 constexpr uint32_t kInfoEnd = 16;                 // k: the worker's last step
 constexpr uint32_t kInfoTile = 32;                // always set
 constexpr int kInfoValid = 8;                     // v: keys that exist, 0 to 64 (8 bits)
-constexpr int kInfoBad = 16;                      // k: blocks of the step outside the cache (8 bits)
+constexpr int kInfoBad = 16;                      // k: blocks of the step outside the cache (16 bits)
 
 // mbar_wait by a whole warp: every lane gets the same answer, so that no lane
 // is left alone at a warp-wide instruction.
