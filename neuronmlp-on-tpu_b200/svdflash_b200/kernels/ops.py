@@ -179,9 +179,10 @@ def workspace_for(device: torch.device, nbytes: int) -> _Workspace:
     A call is several launches that meet in the workspace, and another thread's
     may come between them on the same stream: each thread has its own, and a new
     one takes over what a thread that has ended left on the stream.  A workspace
-    that a capture has used stays alive when a larger one replaces it.  A capture
-    that needs more than there is gets one of its own: it cannot wait for the
-    stream."""
+    that a capture has used stays alive when a larger one replaces it; its graph
+    still shares it with the thread's calls and other graphs of that stream, so
+    replays and such calls follow one another.  A capture that needs more than
+    there is gets one of its own: it cannot wait for the stream."""
     index, stream = device.index, _raw_stream(device.index)
     key = index, stream, threading.get_ident()
     capture = _capture_id(index, stream)
