@@ -154,3 +154,34 @@ def test_a_masked_tree_of_more_than_64_tokens_is_refused(cuda_device, model):
     dec.step(_hidden(91, 64), [64], tree_mask=mask[:64])
     dec.step(_hidden(91, 70), [70])                      # a chain has no such end
     dec.check()
+
+
+def test_a_captured_tree_step_goes_on(cuda_device, model):
+    """Depths come from the mask at every replay: the mask's contents may change between them."""
+    from svdflash_b200.models import PagedDecoder
+    layers, _, _ = model
+    decs = [PagedDecoder(layers, 2, 30, 128) for _ in range(2)]
+    x = _hidden(95, 60)
+    for dec in decs:
+        dec.prefill(x[:30], [20, 10])
+    masks = [torch.tensor(m, dtype=torch.int64, device="cuda") for m in
+             ([1, 3, 5, 9, 1, 2, 6], [1, 2, 5, 13, 1, 3, 7], [1, 3, 7, 15, 1, 3, 5])]
+    feed, mask, news = x[30:37].clone(), masks[0].clone(), [4, 3]
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        first = decs[0].step(feed, news, tree_mask=mask)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            y = decs[0].step(feed, news, tree_mask=mask)
+    assert torch.equal(first, decs[1].step(feed, news, tree_mask=masks[0]))
+    kept = torch.tensor([21, 11], dtype=torch.int32, device="cuda")   # each draft is taken back to one token
+    for i, m in enumerate(masks):
+        for dec in decs:
+            dec.keep(kept + i)
+        feed.copy_(x[37 + 7 * i:44 + 7 * i])
+        mask.copy_(m)
+        graph.replay()
+        assert torch.equal(y, decs[1].step(feed, news, tree_mask=m))
+    decs[0].check()
+    assert decs[0].seq_lens.tolist() == decs[1].seq_lens.tolist() == [27, 16]
